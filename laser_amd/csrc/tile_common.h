@@ -114,17 +114,10 @@ __device__ __forceinline__ float online_softmax_step(f32x16 &st, float &m_run, f
     return alpha;
 }
 
-// o *= alpha on the packed fp32 multiplier (two registers per instruction)
+// o *= alpha
 __device__ __forceinline__ void scale_acc(f32x16 &o, float alpha) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    const f32x2 a2 = {alpha, alpha};
 #pragma unroll
-    for (int g = 0; g < 16; g += 2) {
-        f32x2 v = {o[g], o[g + 1]};
-        v = v * a2;
-        o[g] = v[0];
-        o[g + 1] = v[1];
-    }
+    for (int g = 0; g < 16; g++) o[g] *= alpha;
 }
 
 }  // namespace sgclip
