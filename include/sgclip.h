@@ -367,6 +367,40 @@ int sgclip_rows_scatter_add(const float *src_dev, const int32_t *idx_dev, int ro
 int sgclip_adamw(float *param_dev, const float *grad_dev, float *m_dev, float *v_dev, int64_t n, float lr,
                  float beta1, float beta2, float eps, float weight_decay, int step, void *stream);
 
+/* ------------------------------------------------------------------------
+ * (7) Linear layers in microscaled 4-bit floats (OCP MX: e2m1 elements, one e8m0 scale per 32 consecutive elements of a
+ * row).  No counterpart in the reference, whose linear layers (nn.Linear in transformers models/clip/modeling_clip.py) run
+ * in fp32; a caller that accepts 4-bit products scores at four times the bf16 matrix rate.
+ *
+ * Storage of a [rows, cols] matrix, kp = cols rounded up to 256: codes u8 [rows][kp/2], element k in byte k/2 with even k
+ * in the low nibble, zero codes behind cols; scales u8 [ceil(rows/64)][kp/32][16][4], the byte of (row, block) at
+ * ((row/64 * (kp/32) + block) * 16 + row%16) * 4 + row%64/16.  Both pointers 16-byte aligned.
+ *
+ * A block's exponent is floor(log2 max|x|) - 2 within -127..127, an element the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (ties
+ * to the even code, larger values to 6) times that power of two; a block that holds an infinity or a NaN reads back as NaN.
+ * ---------------------------------------------------------------------- */
+size_t sgclip_mxfp4_codes_bytes(int rows, int cols);
+size_t sgclip_mxfp4_scales_bytes(int rows, int cols);
+/* x bf16 or f32 [rows, cols], row stride ldx elements (any alignment; 16-byte rows are faster). */
+int sgclip_mxfp4_quantize(const void *x_dev, int x_dtype, int64_t ldx, int rows, int cols, void *codes_dev, void *scales_dev,
+                          void *stream);
+/* Back to bf16 (exact): out [rows, cols] with row stride ldo, or, transpose, out [cols, ldo] with out[k][r] = x[r][k], zeros
+ * in columns rows..ldo-1, rows <= ldo <= rows rounded up to 64. */
+int sgclip_mxfp4_dequantize(const void *codes_dev, const void *scales_dev, int rows, int cols, int transpose, void *out_dev,
+                            int64_t ldo, void *stream);
+/* out [M, N] (row stride ldo) = epilogue(x w^T + bias) for quantised x [M, K] and w [N, K], fp32 accumulation; bias f32 [N] or
+ * NULL.  epilogue: SGCLIP_EPI_BIAS_BF16, SGCLIP_EPI_BIAS_GELU_BF16 or SGCLIP_EPI_BIAS_RESID_F32 (out f32 = aux + .., aux f32
+ * [M, N] with row stride ldaux; it may be out itself). */
+int sgclip_mxfp4_gemm(const void *x_codes_dev, const void *x_scales_dev, const void *w_codes_dev, const void *w_scales_dev, int M,
+                      int N, int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev,
+                      int64_t ldo, void *stream);
+/* The same for x bf16 or f32, quantised on the way.  Up to SGCLIP_MXFP4_FEW_ROWS rows need no workspace and one launch. */
+#define SGCLIP_MXFP4_FEW_ROWS 16
+size_t sgclip_mxfp4_linear_workspace_bytes(int M, int K);
+int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void *w_codes_dev, const void *w_scales_dev, int M, int N,
+                        int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
+                        void *workspace_dev, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -118,6 +118,15 @@ SIGNATURES = {
     "sgclip_rows_scatter_add": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "sgclip_adamw": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_float, C.c_float,
                                C.c_float, C.c_float, C.c_int, C.c_void_p]),
+    "sgclip_mxfp4_codes_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "sgclip_mxfp4_scales_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "sgclip_mxfp4_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sgclip_mxfp4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sgclip_mxfp4_gemm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
+                                    C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sgclip_mxfp4_linear_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "sgclip_mxfp4_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 

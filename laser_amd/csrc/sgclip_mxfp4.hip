@@ -1,0 +1,549 @@
+// Microscaled 4-bit floats (OCP MX: e2m1 elements, one e8m0 scale per 32 consecutive elements of a row): quantisation,
+// the way back, and the linear layer  y = epilogue(x W^T + bias)  on v_mfma_scale_f32_16x16x128_f8f6f4.
+//
+// Storage of a [rows, cols] matrix, kp = cols rounded up to 256 (zero codes behind cols):
+//   codes   u8 [rows][kp / 2], element k in byte k / 2, even k in the low nibble;
+//   scales  u8 [ceil(rows / 64)][kp / 32][16][4]: the byte of (row, block) is
+//           ((row / 64 * (kp / 32) + block) * 16 + row % 16) * 4 + row % 64 / 16.
+// A 256-element step of a row is one 128-byte cache line, the unit of the LDS-DMA fetches below.  A lane of the 16 x 16 x 128
+// instruction holds 32 consecutive elements of one row = one scale block; with this scale order the 64 lanes of a wave read
+// the scales of 64 rows x 4 blocks as one contiguous 256-byte load, and the instruction picks the byte of its 16 rows itself.
+#include "tile_common.h"
+
+#include <type_traits>
+
+namespace sgclip {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int MX_K = 256;   // elements per stage and the padding of a row
+
+__host__ __device__ static inline long long mx_kp(int cols) { return ((long long)cols + MX_K - 1) / MX_K * MX_K; }
+
+__device__ __forceinline__ float mx_scale_value(unsigned byte) {   // 2^(byte - 127); 255 = NaN
+    return byte == 255u ? __builtin_nanf("") : __uint_as_float(byte == 0u ? 0x00400000u : byte << 23);
+}
+
+// The block's scale byte from the largest absolute bit pattern of its elements (as f32): floor(log2 max) - 2 + 127, at least
+// 0; a block that holds an infinity or a NaN gets 255.  The IEEE exponent field is floor(log2) + 127 for normal numbers, and
+// subnormal ones fall below the smallest scale anyway.
+__device__ __forceinline__ unsigned mx_scale_byte(unsigned amax_bits) {
+    const unsigned ex = amax_bits >> 23;
+    return ex == 255u ? 255u : (ex > 2u ? ex - 2u : 0u);
+}
+
+// Eight elements to eight codes (element 0 in the low nibble).  x * 2^(127 - byte) is exact wherever it decides a rounding (a
+// product that underflows is far below the smallest code's border), so the conversion's round-to-nearest-even is the format's.
+__device__ __forceinline__ unsigned mx_codes8(const float (&v)[8], unsigned byte) {
+    const float inv = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+    unsigned r = 0;
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) s[j] = byte == 255u ? 0.f : v[j] * inv;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, s[0], s[1], 1.0f, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, s[2], s[3], 1.0f, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, s[4], s[5], 1.0f, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, s[6], s[7], 1.0f, 3);
+    return r;
+}
+
+// Eight elements from column k of a row (zeros behind cols).  VEC: 16-byte loads, whole groups of eight only.
+template <typename T, bool VEC>
+__device__ __forceinline__ void mx_load8(const T *__restrict__ row, int k, int cols, float (&v)[8]) {
+    if constexpr (VEC) {
+        if (k < cols) {
+            if constexpr (std::is_same<T, float>::value) {
+                const float4 a = *(const float4 *)(row + k), b = *(const float4 *)(row + k + 4);
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            } else {
+                const bf16x8 a = *(const bf16x8 *)(row + k);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = (float)a[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = k + j < cols ? (float)row[k + j] : 0.f;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Quantisation: a workgroup takes 64 rows x 256 columns, so that the tile's scales are 512 contiguous bytes; four lanes share
+// a block of 32 and find its maximum with two exchanges.  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written
+// per element.
+// ---------------------------------------------------------------------------
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, long long ldx, int rows, int cols,
+                                                          unsigned char *__restrict__ codes, unsigned char *__restrict__ scales) {
+    __shared__ unsigned char sc[512];
+    const int tid = threadIdx.x;
+    const long long kp = mx_kp(cols);
+    const int kt = (int)(kp / MX_K);
+    const int rb = blockIdx.x / kt, kb = blockIdx.x % kt;
+    const int c = tid & 31, k = kb * MX_K + c * 8;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int row = rb * 64 + (tid >> 5) + 8 * i;
+        if (row < rows) mx_load8<T, VEC>(x + row * ldx, k, cols, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int lr = (tid >> 5) + 8 * i, row = rb * 64 + lr;
+        if (row >= rows) {   // scales behind the last row are read with the tile: keep them defined
+            if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = 0;
+            continue;
+        }
+        unsigned am = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        am = max(am, (unsigned)__shfl_xor((int)am, 1, 64));
+        am = max(am, (unsigned)__shfl_xor((int)am, 2, 64));
+        const unsigned byte = mx_scale_byte(am);
+        *(unsigned *)(codes + row * (kp / 2) + (k >> 1)) = mx_codes8(v[i], byte);
+        if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = (unsigned char)byte;
+    }
+    __syncthreads();
+    if (tid < 128) ((unsigned *)(scales + ((long long)rb * (kp / 32) + kb * 8) * 64))[tid] = ((const unsigned *)sc)[tid];
+}
+
+// ---------------------------------------------------------------------------
+// Back to bf16, which holds every value of the format exactly.  Plain: one thread per eight elements.  Transposed: 64 x 64
+// tiles through LDS, out[k][row] with zeros in columns rows .. ldo - 1 (the reduction padding of the products that follow).
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void mx_values8(unsigned r, float scale, float (&v)[8]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, 1.0f, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, 1.0f, 3);
+    v[0] = a[0] * scale; v[1] = a[1] * scale; v[2] = b[0] * scale; v[3] = b[1] * scale;
+    v[4] = c[0] * scale; v[5] = c[1] * scale; v[6] = d[0] * scale; v[7] = d[1] * scale;
+}
+
+__device__ __forceinline__ float mx_row_scale(const unsigned char *scales, long long kp, long long row, int block) {
+    return mx_scale_value(scales[(((row >> 6) * (kp / 32) + block) * 16 + (row & 15)) * 4 + ((row & 63) >> 4)]);
+}
+
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
+                                                            int rows, int cols, bf16_t *__restrict__ out, long long ldo, int vec) {
+    const long long kp = mx_kp(cols);
+    const int per = (cols + 7) / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)rows * per) return;
+    const long long row = i / per;
+    const int k = (int)(i - row * per) * 8;
+    float v[8];
+    mx_values8(*(const unsigned *)(codes + row * (kp / 2) + (k >> 1)), mx_row_scale(scales, kp, row, k >> 5), v);
+    bf16_t *o = out + row * ldo + k;
+    if (vec) {
+        bf16x8 b;
+#pragma unroll
+        for (int j = 0; j < 8; j++) b[j] = (bf16_t)v[j];
+        *(bf16x8 *)o = b;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (k + j < cols) o[j] = (bf16_t)v[j];
+    }
+}
+
+__global__ __launch_bounds__(256) void mx_dequantize_t_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
+                                                              int rows, int cols, bf16_t *__restrict__ out, long long ldo) {
+    __shared__ bf16_t tile[64][66];
+    const long long kp = mx_kp(cols);
+    const int kt = (cols + 63) / 64;
+    const int r0 = blockIdx.x / kt * 64, k0 = blockIdx.x % kt * 64;
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const int lr = (tid >> 3) + 32 * p, k = k0 + (tid & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = 0.f;
+        if (r0 + lr < rows)
+            mx_values8(*(const unsigned *)(codes + (long long)(r0 + lr) * (kp / 2) + (k >> 1)), mx_row_scale(scales, kp, r0 + lr, k >> 5), v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) tile[lr][(tid & 7) * 8 + j] = (bf16_t)v[j];
+    }
+    __syncthreads();
+    const int c = tid & 63;
+#pragma unroll
+    for (int p = 0; p < 16; p++) {
+        const int k = (tid >> 6) + 4 * p;
+        if (k0 + k < cols && r0 + c < ldo) out[(long long)(k0 + k) * ldo + r0 + c] = tile[c][k];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The product.  The weights are the instruction's first operand: a lane's four results are four consecutive columns of one
+// row of y.
+// ---------------------------------------------------------------------------
+struct MxGemm {
+    const unsigned char *xc, *xs, *wc, *ws;   // codes and scales of x [M, K] and w [N, K]
+    const float *bias, *resid;
+    void *out;
+    long long ldr, ldo, kp;
+    int M, N;
+    int wide;    // out, bias, resid allow four columns per access
+};
+
+__device__ __forceinline__ float mx_gelu(float x) { return x / (1.0f + __expf(-1.702f * x)); }
+
+enum { MX_BF16 = 0, MX_GELU = 1, MX_RESID = 2 };
+
+// four consecutive columns n .. n + 3 of row m
+template <int EPI>
+__device__ __forceinline__ void mx_store4(const MxGemm &g, f32x4 v, int m, int n) {
+    if (m >= g.M || n >= g.N) return;
+    if (g.wide) {   // N % 4 == 0: the four columns are all inside
+        if (g.bias) {
+            const float4 b = *(const float4 *)(g.bias + n);
+            v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+        }
+        if constexpr (EPI == MX_RESID) {
+            const float4 r = *(const float4 *)(g.resid + m * g.ldr + n);
+            *(float4 *)((float *)g.out + m * g.ldo + n) = make_float4(r.x + v[0], r.y + v[1], r.z + v[2], r.w + v[3]);
+        } else {
+            bf16x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v[j]) : v[j]);
+            *(bf16x4 *)((bf16_t *)g.out + m * g.ldo + n) = o;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (n + j >= g.N) break;
+        const float t = v[j] + (g.bias ? g.bias[n + j] : 0.f);
+        if constexpr (EPI == MX_RESID) ((float *)g.out)[m * g.ldo + n + j] = g.resid[m * g.ldr + n + j] + t;
+        else ((bf16_t *)g.out)[m * g.ldo + n + j] = (bf16_t)(EPI == MX_GELU ? mx_gelu(t) : t);
+    }
+}
+
+template <int I, int N, typename F>
+__device__ __forceinline__ void static_for(F &&f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
+
+__device__ __forceinline__ i32x8 mx_operand(i32x4 v) { return (i32x8){v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
+
+// Tile of 2 WT x 2 WT, four waves of WT x WT (32 or 64) each; one 256-deep stage in flight behind the one computed, one barrier
+// per stage.
+template <int EPI, int WT>
+__global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
+    constexpr int T = 2 * WT, NT = WT / 16, OP = T * 128;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1, r = lane & 15, q = lane >> 4;
+    const int tiles_n = (g.N + T - 1) / T, ntiles = gridDim.x;
+    const int swz = xcd_remap(blockIdx.x, ntiles);
+    const int m0 = swz / tiles_n * T, n0 = swz % tiles_n * T;
+    const long long ld = g.kp / 2;
+    const int ns = (int)(g.kp / MX_K);
+
+    auto fetch = [&](int s, unsigned char *slot) {
+#pragma unroll
+        for (int p = wave; p < T / 8; p += 4) {
+            const int row = p * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+            const unsigned char *sx = g.xc + min(m0 + row, g.M - 1) * ld + s * 128 + c * 16;
+            const unsigned char *sw = g.wc + min(n0 + row, g.N - 1) * ld + s * 128 + c * 16;
+            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sx), LDS_PTR(slot + p * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sw), LDS_PTR(slot + OP + p * 1024), 16, 0, 0);
+        }
+    };
+    // scale rows of this wave: group of 64 rows (the last one where the tile hangs over), first 16-row byte inside it
+    const int mrow = m0 + wm * WT, nrow = n0 + wn * WT;
+    const unsigned char *xs = g.xs + (long long)min(mrow >> 6, (g.M - 1) >> 6) * (g.kp / 32) * 64;
+    const unsigned char *wsc = g.ws + (long long)min(nrow >> 6, (g.N - 1) >> 6) * (g.kp / 32) * 64;
+    const int xsh = (mrow & 63) / 16 * 8, wsh = (nrow & 63) / 16 * 8;
+
+    f32x4 acc[NT][NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    fetch(0, lds);
+    for (int s = 0; s < ns; s++) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const unsigned char *cur = lds + (s & 1) * 2 * OP;
+        unsigned sa[2], sb[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            sa[t] = *(const unsigned *)(wsc + ((s * 8 + t * 4 + q) * 16 + r) * 4) >> wsh;
+            sb[t] = *(const unsigned *)(xs + ((s * 8 + t * 4 + q) * 16 + r) * 4) >> xsh;
+        }
+        if (s + 1 < ns) fetch(s + 1, lds + ((s + 1) & 1) * 2 * OP);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            i32x4 fx[NT], fw[NT];
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                fx[i] = *(const i32x4 *)(cur + lds_off(wm * WT + i * 16 + r, t * 4 + q));
+                fw[i] = *(const i32x4 *)(cur + OP + lds_off(wn * WT + i * 16 + r, t * 4 + q));
+            }
+            static_for<0, NT>([&](auto ic) {
+                static_for<0, NT>([&](auto jc) {
+                    constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fw[j]), mx_operand(fx[i]), acc[i][j], 4, 4, j,
+                                                                                 (int)sa[t], i, (int)sb[t]);
+                });
+            });
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) mx_store4<EPI>(g, acc[i][j], mrow + i * 16 + r, nrow + j * 16 + q * 4);
+}
+
+// Up to 16 rows of x, quantised on the way in: a workgroup takes 16 columns of y, its eight waves 128-deep slices of K in turn,
+// and joins their sums through LDS.  A lane holds one block of 32 of one row, so the block's maximum needs no exchange.
+// Bound by the weights' bytes (and, below about a megabyte of them, by the launch).
+template <typename T, bool VEC, int EPI>
+__global__ __launch_bounds__(512) void mx_few_rows_kernel(const T *__restrict__ x, long long ldx, int K, MxGemm g) {
+    __shared__ f32x4 part[8][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const long long ld = g.kp / 2;
+    const int nrow = min(n0 + r, g.N - 1);
+    const unsigned char *wc = g.wc + nrow * ld;
+    f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int steps = (K + 127) / 128;
+    for (int s = wave; s < steps; s += 8) {
+        const int block = s * 4 + q;
+        const i32x4 fw = *(const i32x4 *)(wc + block * 16);
+        const unsigned sw = g.ws[(((long long)(nrow >> 6) * (g.kp / 32) + block) * 16 + (nrow & 15)) * 4 + ((nrow & 63) >> 4)];
+        i32x4 fx = (i32x4){0, 0, 0, 0};
+        unsigned sx = 0;
+        if (r < g.M) {
+            float v[4][8];
+            unsigned am = 0;
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                mx_load8<T, VEC>(x + r * ldx, block * 32 + p * 8, K, v[p]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[p][j]) & 0x7fffffffu);
+            }
+            sx = mx_scale_byte(am);
+#pragma unroll
+            for (int p = 0; p < 4; p++) fx[p] = (int)mx_codes8(v[p], sx);
+        }
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fw), mx_operand(fx), acc, 4, 4, 0, (int)sw, 0, (int)sx);
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < 8; w++) acc += part[w][lane];
+        mx_store4<EPI>(g, acc, r, n0 + q * 4);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static bool mx_shape_ok(const char *who, int rows, int cols) {
+    if (rows < 0 || rows > (1 << 30) || cols <= 0 || cols > (1 << 24)) {
+        set_error("%s: bad shape rows=%d cols=%d", who, rows, cols);
+        return false;
+    }
+    return true;
+}
+
+// a launch counts its threads in 32 bits
+static bool mx_grid_ok(const char *who, long long blocks, int threads) {
+    if (blocks * threads > 0xffffffffLL) {
+        set_error("%s: %lld workgroups of %d threads are more than one launch holds", who, blocks, threads);
+        return false;
+    }
+    return true;
+}
+
+static bool mx_storage_ok(const char *who, const void *codes, const void *scales) {
+    if (!codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15)) {
+        set_error("%s: codes and scales must be 16-byte aligned device pointers", who);
+        return false;
+    }
+    return true;
+}
+
+template <typename T>
+static int mx_launch_quantize(const T *x, long long ldx, int rows, int cols, unsigned char *codes, unsigned char *scales, hipStream_t stream) {
+    const bool vec = cols % 8 == 0 && ldx * sizeof(T) % 16 == 0 && ((uintptr_t)x & 15) == 0;
+    const long long blocks = ((long long)rows + 63) / 64 * (mx_kp(cols) / MX_K);
+    if (!mx_grid_ok("sgclip_mxfp4_quantize", blocks, 256)) return SGCLIP_EINVAL;
+    if (vec) mx_quantize_kernel<T, true><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+    else mx_quantize_kernel<T, false><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+    return launch_check("sgclip_mxfp4_quantize");
+}
+
+template <int EPI>
+static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
+    // 128 x 128 tiles where they fill the chip, 64 x 64 below that
+    const long long big = (((long long)g.M + 127) / 128) * (((long long)g.N + 127) / 128);
+    if (!mx_grid_ok("sgclip_mxfp4_gemm", big, 256)) return SGCLIP_EINVAL;
+    if (big >= device_cus()) {
+        if (!lds_attr((const void *)mx_gemm_kernel<EPI, 64>, 4 * 128 * 128)) return SGCLIP_ELAUNCH;
+        mx_gemm_kernel<EPI, 64><<<dim3((unsigned)big), 256, 4 * 128 * 128, stream>>>(g);
+    } else {
+        const long long small = (((long long)g.M + 63) / 64) * (((long long)g.N + 63) / 64);
+        mx_gemm_kernel<EPI, 32><<<dim3((unsigned)small), 256, 4 * 64 * 128, stream>>>(g);
+    }
+    return SGCLIP_OK;
+}
+
+template <typename T, int EPI>
+static void mx_launch_few(const T *x, long long ldx, int K, const MxGemm &g, hipStream_t stream) {
+    const bool vec = K % 8 == 0 && ldx * sizeof(T) % 16 == 0 && ((uintptr_t)x & 15) == 0;
+    const dim3 grid((unsigned)((g.N + 15) / 16));
+    if (vec) mx_few_rows_kernel<T, true, EPI><<<grid, 512, 0, stream>>>(x, ldx, K, g);
+    else mx_few_rows_kernel<T, false, EPI><<<grid, 512, 0, stream>>>(x, ldx, K, g);
+}
+
+static int mx_epilogue(const char *who, MxGemm &g, int epilogue, const float *bias, const float *aux, int64_t ldaux, void *out, int64_t ldo,
+                       int &epi) {
+    switch (epilogue) {
+        case SGCLIP_EPI_BIAS_BF16: epi = MX_BF16; break;
+        case SGCLIP_EPI_BIAS_GELU_BF16: epi = MX_GELU; break;
+        case SGCLIP_EPI_BIAS_RESID_F32: epi = MX_RESID; break;
+        default: set_error("%s: epilogue %d is not one of the 4-bit product's", who, epilogue); return SGCLIP_EINVAL;
+    }
+    if (!out || ldo < g.N || (epi == MX_RESID && (!aux || ldaux < g.N))) {
+        set_error("%s: output / residual missing or its row stride below N=%d", who, g.N);
+        return SGCLIP_EINVAL;
+    }
+    g.bias = bias;
+    g.resid = epi == MX_RESID ? aux : nullptr;
+    g.ldr = ldaux;
+    g.out = out;
+    g.ldo = ldo;
+    g.wide = g.N % 4 == 0 && ldo % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)bias & 15) == 0 &&
+             (epi != MX_RESID || (ldaux % 4 == 0 && ((uintptr_t)aux & 15) == 0));
+    return SGCLIP_OK;
+}
+
+}  // namespace sgclip
+
+using namespace sgclip;
+
+extern "C" {
+
+size_t sgclip_mxfp4_codes_bytes(int rows, int cols) { return rows <= 0 || cols <= 0 ? 0 : (size_t)rows * (size_t)(mx_kp(cols) / 2); }
+
+size_t sgclip_mxfp4_scales_bytes(int rows, int cols) {
+    return rows <= 0 || cols <= 0 ? 0 : ((size_t)rows + 63) / 64 * 64 * (size_t)(mx_kp(cols) / 32);
+}
+
+int sgclip_mxfp4_quantize(const void *x_dev, int x_dtype, int64_t ldx, int rows, int cols, void *codes_dev, void *scales_dev, void *stream) {
+    if (!mx_shape_ok("sgclip_mxfp4_quantize", rows, cols)) return SGCLIP_EINVAL;
+    if (rows == 0) return SGCLIP_OK;
+    if (!x_dev || ldx < cols || (x_dtype != SGCLIP_DTYPE_F32 && x_dtype != SGCLIP_DTYPE_BF16)) {
+        set_error("sgclip_mxfp4_quantize: bad x (dtype %d, row stride %lld, cols %d)", x_dtype, (long long)ldx, cols);
+        return SGCLIP_EINVAL;
+    }
+    if (!mx_storage_ok("sgclip_mxfp4_quantize", codes_dev, scales_dev)) return SGCLIP_EINVAL;
+    unsigned char *c = (unsigned char *)codes_dev, *s = (unsigned char *)scales_dev;
+    return x_dtype == SGCLIP_DTYPE_F32 ? mx_launch_quantize((const float *)x_dev, ldx, rows, cols, c, s, (hipStream_t)stream)
+                                       : mx_launch_quantize((const bf16_t *)x_dev, ldx, rows, cols, c, s, (hipStream_t)stream);
+}
+
+int sgclip_mxfp4_dequantize(const void *codes_dev, const void *scales_dev, int rows, int cols, int transpose, void *out_dev, int64_t ldo,
+                            void *stream) {
+    if (!mx_shape_ok("sgclip_mxfp4_dequantize", rows, cols)) return SGCLIP_EINVAL;
+    if (rows == 0) return SGCLIP_OK;
+    if (!out_dev || ldo < (transpose ? rows : cols) || (transpose && ldo > ((int64_t)rows + 63) / 64 * 64)) {
+        set_error("sgclip_mxfp4_dequantize: bad output row stride %lld for rows=%d cols=%d transpose=%d", (long long)ldo, rows, cols, transpose);
+        return SGCLIP_EINVAL;
+    }
+    if (!mx_storage_ok("sgclip_mxfp4_dequantize", codes_dev, scales_dev)) return SGCLIP_EINVAL;
+    const unsigned char *c = (const unsigned char *)codes_dev, *s = (const unsigned char *)scales_dev;
+    if (transpose) {
+        const long long tiles = (((long long)rows + 63) / 64) * ((cols + 63) / 64);
+        if (!mx_grid_ok("sgclip_mxfp4_dequantize", tiles, 256)) return SGCLIP_EINVAL;
+        mx_dequantize_t_kernel<<<dim3((unsigned)tiles), 256, 0, (hipStream_t)stream>>>(c, s, rows, cols, (bf16_t *)out_dev, ldo);
+    } else {
+        const int vec = cols % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)out_dev & 15) == 0;
+        const long long n = (long long)rows * ((cols + 7) / 8);
+        if (!mx_grid_ok("sgclip_mxfp4_dequantize", (n + 255) / 256, 256)) return SGCLIP_EINVAL;
+        mx_dequantize_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, (hipStream_t)stream>>>(c, s, rows, cols, (bf16_t *)out_dev, ldo, vec);
+    }
+    return launch_check("sgclip_mxfp4_dequantize");
+}
+
+int sgclip_mxfp4_gemm(const void *x_codes_dev, const void *x_scales_dev, const void *w_codes_dev, const void *w_scales_dev, int M, int N,
+                      int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
+                      void *stream) {
+    if (!mx_shape_ok("sgclip_mxfp4_gemm", M, K) || !mx_shape_ok("sgclip_mxfp4_gemm", N, K)) return SGCLIP_EINVAL;
+    if (M == 0 || N == 0) return SGCLIP_OK;
+    if (!mx_storage_ok("sgclip_mxfp4_gemm", x_codes_dev, x_scales_dev) || !mx_storage_ok("sgclip_mxfp4_gemm", w_codes_dev, w_scales_dev))
+        return SGCLIP_EINVAL;
+    MxGemm g{};
+    g.xc = (const unsigned char *)x_codes_dev;
+    g.xs = (const unsigned char *)x_scales_dev;
+    g.wc = (const unsigned char *)w_codes_dev;
+    g.ws = (const unsigned char *)w_scales_dev;
+    g.M = M;
+    g.N = N;
+    g.kp = mx_kp(K);
+    int epi;
+    int rc = mx_epilogue("sgclip_mxfp4_gemm", g, epilogue, bias_dev, aux_dev, ldaux, out_dev, ldo, epi);
+    if (rc != SGCLIP_OK) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    rc = epi == MX_BF16 ? mx_launch_gemm<MX_BF16>(g, st) : epi == MX_GELU ? mx_launch_gemm<MX_GELU>(g, st) : mx_launch_gemm<MX_RESID>(g, st);
+    return rc != SGCLIP_OK ? rc : launch_check("sgclip_mxfp4_gemm");
+}
+
+size_t sgclip_mxfp4_linear_workspace_bytes(int M, int K) {
+    if (M <= SGCLIP_MXFP4_FEW_ROWS) return 0;
+    return align_up(sgclip_mxfp4_codes_bytes(M, K), 256) + sgclip_mxfp4_scales_bytes(M, K);
+}
+
+int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void *w_codes_dev, const void *w_scales_dev, int M, int N, int K,
+                        int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
+                        void *workspace_dev, size_t workspace_bytes, void *stream) {
+    if (!mx_shape_ok("sgclip_mxfp4_linear", M, K) || !mx_shape_ok("sgclip_mxfp4_linear", N, K)) return SGCLIP_EINVAL;
+    if (M == 0 || N == 0) return SGCLIP_OK;
+    if (M > SGCLIP_MXFP4_FEW_ROWS) {
+        if (workspace_bytes < sgclip_mxfp4_linear_workspace_bytes(M, K) || !workspace_dev) {
+            set_error("sgclip_mxfp4_linear: workspace of %zu bytes, %zu needed", workspace_bytes, sgclip_mxfp4_linear_workspace_bytes(M, K));
+            return SGCLIP_ENOSPC;
+        }
+        unsigned char *codes = (unsigned char *)workspace_dev, *scales = codes + align_up(sgclip_mxfp4_codes_bytes(M, K), 256);
+        const int rc = sgclip_mxfp4_quantize(x_dev, x_dtype, ldx, M, K, codes, scales, stream);
+        if (rc != SGCLIP_OK) return rc;
+        return sgclip_mxfp4_gemm(codes, scales, w_codes_dev, w_scales_dev, M, N, K, epilogue, bias_dev, aux_dev, ldaux, out_dev, ldo, stream);
+    }
+    if (!x_dev || ldx < K || (x_dtype != SGCLIP_DTYPE_F32 && x_dtype != SGCLIP_DTYPE_BF16)) {
+        set_error("sgclip_mxfp4_linear: bad x (dtype %d, row stride %lld, K %d)", x_dtype, (long long)ldx, K);
+        return SGCLIP_EINVAL;
+    }
+    if (!mx_storage_ok("sgclip_mxfp4_linear", w_codes_dev, w_scales_dev)) return SGCLIP_EINVAL;
+    MxGemm g{};
+    g.wc = (const unsigned char *)w_codes_dev;
+    g.ws = (const unsigned char *)w_scales_dev;
+    g.M = M;
+    g.N = N;
+    g.kp = mx_kp(K);
+    int epi;
+    const int rc = mx_epilogue("sgclip_mxfp4_linear", g, epilogue, bias_dev, aux_dev, ldaux, out_dev, ldo, epi);
+    if (rc != SGCLIP_OK) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    const bool f32 = x_dtype == SGCLIP_DTYPE_F32;
+    const float *xf = (const float *)x_dev;
+    const bf16_t *xb = (const bf16_t *)x_dev;
+    if (epi == MX_BF16) f32 ? mx_launch_few<float, MX_BF16>(xf, ldx, K, g, st) : mx_launch_few<bf16_t, MX_BF16>(xb, ldx, K, g, st);
+    else if (epi == MX_GELU) f32 ? mx_launch_few<float, MX_GELU>(xf, ldx, K, g, st) : mx_launch_few<bf16_t, MX_GELU>(xb, ldx, K, g, st);
+    else f32 ? mx_launch_few<float, MX_RESID>(xf, ldx, K, g, st) : mx_launch_few<bf16_t, MX_RESID>(xb, ldx, K, g, st);
+    return launch_check("sgclip_mxfp4_linear");
+}
+
+}  // extern "C"

@@ -6,12 +6,12 @@ train step's backward pass is one of the calls below (or `ops.gemm_bf16`).
 from __future__ import annotations
 
 import os
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from .ops import _ptr, _stream, gemm_bf16
+from .ops import Mxfp4, _ptr, _same_device, _stream, dequantize_mxfp4, gemm_bf16
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -247,3 +247,43 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: Optional[torch.Tensor] 
     dyt = transpose_bf16(dy, Mp)
     xt = transpose_bf16(x, Mp)
     return gemm_bf16(dyt, xt, out, _lib.EPI_F32_ATOMIC)
+
+
+# -- linear layers in 4-bit floats -----------------------------------------------------------
+def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dtype = BF16, need_dx: bool = True, need_dw: bool = True,
+                     need_db: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dw, db) of y = xq wq^T + b for dy bf16 / f32 [M, N]: the gradient in the quantised operands, which a straight-through
+    estimator hands to the unquantised ones.  dx [M, K] in dx_dtype, dw f32 [N, K], db f32 [N]; what is not needed is None.
+    dy enters the products in bf16; the 4-bit operands enter exactly.  dw is summed with fp32 atomics (`linear_wgrad`)."""
+    if dy.dim() != 2 or dy.dtype not in (BF16, F32) or dy.shape != (xq.rows, wq.rows) or xq.cols != wq.cols:
+        raise ValueError(f"linear_mxfp4_bwd: dy {dy.dtype} {tuple(dy.shape)} for x {xq.shape} and weight {wq.shape}")
+    if dx_dtype not in (BF16, F32):
+        raise ValueError(f"linear_mxfp4_bwd: dx in {dx_dtype}")
+    _same_device(dy, xq.codes, wq.codes)
+    dy = dy.contiguous()
+    M, N, K = xq.rows, wq.rows, xq.cols
+    dev = dy.device
+    db = torch.zeros(N, dtype=F32, device=dev) if need_db else None
+    if M == 0:
+        return (torch.empty((0, K), dtype=dx_dtype, device=dev) if need_dx else None,
+                torch.zeros((N, K), dtype=F32, device=dev) if need_dw else None, db)
+    if dy.dtype == F32:
+        dyb = cast_bf16_colsum(dy, db) if need_db else cast_bf16(dy)
+    else:
+        dyb = dy
+        if need_db:
+            colsum(dy, db)
+    dx = None
+    if need_dx:
+        w_t = dequantize_mxfp4(wq, transpose=True)       # [K, N rounded up to 64], zeros behind N
+        dyp = dyb
+        if w_t.shape[1] != N:
+            dyp = torch.zeros((M, w_t.shape[1]), dtype=BF16, device=dev)
+            dyp[:, :N] = dyb
+        dx = torch.empty((M, K), dtype=dx_dtype, device=dev)
+        if dx_dtype == F32:
+            gemm_bf16(dyp, w_t, dx, _lib.EPI_F32)
+        else:
+            gemm_bf16(dyp, w_t, dx, _lib.EPI_BIAS_BF16, bias=torch.zeros(K, dtype=F32, device=dev))
+    dw = linear_wgrad(dyb, dequantize_mxfp4(xq)) if need_dw else None
+    return dx, dw, db

@@ -503,6 +503,40 @@ def segment_mean(probs: torch.Tensor, seg: torch.Tensor, n_groups: int, seg_host
     return _SegmentMeanFn.apply(probs, seg, inv, n_groups)
 
 
+class _LinearMxfp4Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(weight)
+        ctx.save_for_backward(xq.codes, xq.scales, wq.codes, wq.scales)
+        ctx.shapes, ctx.dtypes = (xq.shape, wq.shape), (x.dtype, weight.dtype)
+        return ops.linear_mxfp4(xq, wq, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xc, xs, wc, ws = ctx.saved_tensors
+        xq, wq = ops.Mxfp4(xc, xs, *ctx.shapes[0]), ops.Mxfp4(wc, ws, *ctx.shapes[1])
+        dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, ctx.dtypes[0], *ctx.needs_input_grad)
+        return dx, dw if dw is None else dw.to(ctx.dtypes[1]), db
+
+
+def linear_mxfp4(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """nn.Linear's product with both operands quantised to microscaled 4-bit floats at every call (`ops.quantize_mxfp4`), and
+    gradients that pass straight through the rounding: what a model is fine-tuned with that `ops.linear_mxfp4` will score.
+    x: bf16 / f32 [..., K]; weight: f32 / bf16 [N, K]; bias: f32 [N] or None; result bf16 [..., N].  Between forward and
+    backward x and the weight are held in 4 bits.  Under graph capture only without gradients: a captured step calls
+    `ops.linear_mxfp4` and `grad_ops.linear_mxfp4_bwd` itself."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)) and \
+            torch.cuda.is_current_stream_capturing():
+        # autograd's own bookkeeping of the leaves may belong to another stream, which a capture does not survive
+        raise RuntimeError("linear_mxfp4 builds no autograd graph under graph capture: call ops.linear_mxfp4 and "
+                           "grad_ops.linear_mxfp4_bwd")
+    y = _LinearMxfp4Fn.apply(x.reshape(-1, x.shape[-1]).contiguous(), weight.contiguous(), bias)
+    return y.view(x.shape[:-1] + (weight.shape[0],))
+
+
 # ---------------------------------------------------------------------------------------------
 # optimizer and gradient exchange
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,274 @@
+"""GPU tests of the microscaled 4-bit linear layers against their definition in 64 bits.
+
+Tolerances.  Quantised operands are exact, and a product of two 4-bit values times powers of two is exact in fp32, so a sum of
+K of them is off by at most K roundings of half a step, K 2^-24 times the sum of the terms' absolute values, whatever the
+order; the bias and the residual add one rounding each.  A result rounded to bf16 adds 2^-8 of its value."""
+import pytest
+import torch
+
+from laser_amd import _lib, grad_ops as G, ops, training
+from mxfp4_ref import values
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+U32, UBF = 2.0 ** -24, 2.0 ** -8
+
+
+def _x(rows, cols, dtype, scale=1.0):
+    x = torch.randn(rows, cols, device="cuda") * scale
+    return (x * (1 + 9 * (torch.rand(cols, device="cuda") < 0.05))).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 32), (3, 31), (2, 33), (64, 256), (65, 257), (130, 1000), (77, 512), (1, 4096)])
+def test_quantize_is_the_definition(rows, cols, dtype):
+    x = _x(rows, cols, dtype)
+    q = ops.quantize_mxfp4(x)
+    got = ops.dequantize_mxfp4(q)
+    assert torch.equal(got.double(), values(x))
+    t = ops.dequantize_mxfp4(q, transpose=True)
+    assert t.shape == (cols, (rows + 63) // 64 * 64)
+    assert torch.equal(t[:, :rows], got.t()) and not t[:, rows:].any()
+    # a second quantisation changes nothing: every value of the format is its own nearest one unless the block's largest
+    # element rounded down across a power of two, which the saturating end of the format excludes
+    assert torch.equal(ops.dequantize_mxfp4(ops.quantize_mxfp4(got)), got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quantize_strided_and_misaligned_rows(dtype):
+    base = _x(40, 700, dtype)
+    for view in (base[:, :512], base[:, 1:513], base[::2, 3:100], base[5:6, 7:8], base[:, :8].as_strided((40, 8), (700, 1), 4)):
+        assert torch.equal(ops.dequantize_mxfp4(ops.quantize_mxfp4(view)).double(), values(view))
+
+
+def test_quantize_every_bf16_value():
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF16).cuda()
+    finite = every[torch.isfinite(every.float())]
+    x = finite[torch.randperm(finite.numel(), device="cuda")][: finite.numel() // 32 * 32].view(-1, 32)
+    assert torch.equal(ops.dequantize_mxfp4(ops.quantize_mxfp4(x)).double(), values(x))
+    # sorted by magnitude: the blocks cover every exponent, the subnormal ones and zero among them
+    x = finite[finite.float().abs().argsort()][: finite.numel() // 32 * 32].view(-1, 32)
+    assert torch.equal(ops.dequantize_mxfp4(ops.quantize_mxfp4(x)).double(), values(x))
+
+
+@pytest.mark.parametrize("top", [1.0, 1.9999999, 7.9e-38, 1.2e-38, 3e-39, 1e-40, 1.4e-45, 1.6e38])
+def test_quantize_borders(top):
+    """Every border between codes, its two neighbours and the block's maximum, at scales up to both ends of the range."""
+    scale = 2.0 ** max(-127, torch.tensor(top, dtype=F64).log2().floor().item() - 2)
+    marks = torch.tensor([0.25, 0.5, 0.75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7], dtype=F64) * scale
+    near = marks.float()
+    near = torch.cat([near, torch.nextafter(near, torch.tensor(0.0)), torch.nextafter(near, torch.tensor(1e38))])
+    near = torch.cat([near[near <= top], torch.tensor([top])])
+    x = torch.zeros(2 * near.numel(), 32)
+    x[:, 0] = top
+    x[: near.numel(), 5], x[near.numel():, 5] = near, -near
+    x = x.cuda()
+    assert torch.equal(ops.dequantize_mxfp4(ops.quantize_mxfp4(x)).double(), values(x).to(BF16).double())
+
+
+def test_not_finite_blocks_read_back_as_nan():
+    x = torch.zeros(4, 70, device="cuda")
+    x[0, 3], x[1, 40], x[2, 69], x[3, 0] = float("nan"), float("inf"), float("-inf"), 3.0
+    got = ops.dequantize_mxfp4(ops.quantize_mxfp4(x))
+    want = torch.zeros(4, 70, dtype=torch.bool, device="cuda")
+    want[0, :32], want[1, 32:64], want[2, 64:] = True, True, True
+    assert torch.equal(torch.isnan(got), want) and got[3, 0] == 3.0
+
+
+def _check(y, ref, size, K, terms, extra=0.0):
+    """|y - ref| <= (K + terms) half steps of the absolute sum + extra."""
+    bound = (K + terms) * U32 * size + extra + 1e-45
+    worst = ((y.double() - ref).abs() - bound).max().item()
+    assert worst <= 0, worst
+
+
+SHAPES = [(1, 1, 1), (1, 64, 32), (3, 5, 33), (7, 1024, 4096), (16, 2048, 512), (17, 100, 300), (64, 64, 256), (65, 63, 255),
+          (130, 257, 515), (300, 300, 1000), (1540, 768, 768), (2100, 2049, 640)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_against_64_bits(M, N, K, dtype):
+    x, w = _x(M, K, dtype), 0.02 * torch.randn(N, K, device="cuda")
+    b, r = torch.randn(N, device="cuda"), torch.randn(M, N, device="cuda")
+    xv, wv = values(x), values(w)
+    s, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    wq = ops.quantize_mxfp4(w)
+    y = ops.linear_mxfp4(x, wq, b, residual=r)
+    assert y.dtype == F32
+    _check(y, r.double() + s + b.double(), size + b.double().abs() + r.double().abs(), K, 2)
+    y = ops.linear_mxfp4(x, wq)
+    assert y.dtype == BF16
+    _check(y, s, size, K, 0, UBF * (s.abs() + K * U32 * size))
+    # quick_gelu's slope is at most 1.1; its own few roundings are far below the bf16 one
+    u = s + b.double()
+    g = u * torch.sigmoid(1.702 * u)
+    err = 1.1 * (K + 1) * U32 * (size + b.double().abs()) + 2.0 ** -20 * g.abs()
+    _check(ops.linear_mxfp4(x, wq, b, gelu=True), g, 0 * size, 0, 0, err + UBF * (g.abs() + err))
+    # operands quantised beforehand give the same sums
+    _check(ops.linear_mxfp4(ops.quantize_mxfp4(x), wq, b, residual=r), r.double() + s + b.double(),
+           size + b.double().abs() + r.double().abs(), K, 2)
+
+
+def test_linear_views_in_place_and_untouched_neighbours():
+    M, N, K = 70, 96, 160
+    x = _x(2 * M, K + 9, BF16)[::2, 5:5 + K]
+    wq = ops.quantize_mxfp4(0.1 * torch.randn(N, K, device="cuda"))
+    b = torch.randn(N, device="cuda")
+    for rows in (M, 5):
+        store = torch.full((rows + 2, N + 6), 7.0, device="cuda")
+        r = store[1:1 + rows, 3:3 + N]
+        r.copy_(torch.randn(rows, N, device="cuda"))
+        want = ops.linear_mxfp4(x[:rows].contiguous(), wq, b, residual=r.clone())
+        got = ops.linear_mxfp4(x[:rows], wq, b, residual=r, out=r)
+        assert got.data_ptr() == r.data_ptr() and torch.equal(got, want)
+        edge = store.clone()
+        edge[1:1 + rows, 3:3 + N] = 7.0
+        assert (edge == 7.0).all()
+
+
+def test_not_finite_operands_reach_their_rows_and_columns_only():
+    x, w = torch.randn(40, 96, device="cuda"), torch.randn(70, 96, device="cuda")
+    x[3, 50], w[9, 1] = float("inf"), float("nan")
+    want = torch.zeros(40, 70, dtype=torch.bool, device="cuda")
+    want[3], want[:, 9] = True, True
+    wq = ops.quantize_mxfp4(w)
+    assert torch.equal(torch.isnan(ops.linear_mxfp4(x, wq)), want)
+    assert torch.equal(torch.isnan(ops.linear_mxfp4(x[:10], wq)), want[:10])
+
+
+def test_empty_and_zero():
+    wq = ops.quantize_mxfp4(torch.randn(5, 64, device="cuda"))
+    assert ops.linear_mxfp4(torch.empty(0, 64, device="cuda"), wq).shape == (0, 5)
+    b = torch.randn(5, device="cuda")
+    assert torch.equal(ops.linear_mxfp4(torch.zeros(40, 64, device="cuda"), wq, b), b.to(BF16).expand(40, 5))
+    none = ops.quantize_mxfp4(torch.empty(0, 64, device="cuda"))
+    assert ops.linear_mxfp4(torch.zeros(40, 64, device="cuda"), none).shape == (40, 0)
+
+
+def test_refusals():
+    x, w = torch.randn(4, 64, device="cuda"), ops.quantize_mxfp4(torch.randn(8, 64, device="cuda"))
+    r, b = torch.randn(4, 8, device="cuda"), torch.randn(8, device="cuda")
+    for bad in (lambda: ops.quantize_mxfp4(x.half()), lambda: ops.quantize_mxfp4(x[0]), lambda: ops.quantize_mxfp4(x.t()),
+                lambda: ops.quantize_mxfp4(x.cpu()), lambda: ops.quantize_mxfp4(x[:, :0]), lambda: ops.quantize_mxfp4(x[:1].expand(4, 64)),
+                lambda: ops.linear_mxfp4(x[:, :63], w), lambda: ops.linear_mxfp4(x, w, b[:7]), lambda: ops.linear_mxfp4(x, w, b.double()),
+                lambda: ops.linear_mxfp4(x, w, gelu=True, residual=r), lambda: ops.linear_mxfp4(x, w, residual=r[:3]),
+                lambda: ops.linear_mxfp4(x, w, residual=r.to(BF16)), lambda: ops.linear_mxfp4(x, w, out=r),
+                lambda: ops.linear_mxfp4(x, w, residual=r, out=torch.empty(4, 9, device="cuda")),
+                lambda: ops.linear_mxfp4(x, w, residual=r, out=x[:, :8]),
+                lambda: ops.linear_mxfp4(x, w, residual=r[1:], out=r[:3]),
+                lambda: ops.Mxfp4(w.codes, w.scales, 8, 300), lambda: ops.Mxfp4(w.codes.float(), w.scales, 8, 64),
+                lambda: training.linear_mxfp4(x, torch.randn(8, 63, device="cuda")),
+                lambda: G.linear_mxfp4_bwd(r, ops.quantize_mxfp4(x), ops.quantize_mxfp4(x))):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    big = torch.randn(32, 64, device="cuda")
+    y = torch.empty(32, 8, dtype=BF16, device="cuda")
+    rc = lib.sgclip_mxfp4_linear(big.data_ptr(), 0, 64, w.codes.data_ptr(), w.scales.data_ptr(), 32, 8, 64, 0, None, None, 0, y.data_ptr(), 8,
+                                 None, 0, st)
+    assert rc == _lib.ENOSPC
+
+
+def test_side_stream_and_replayed_graph():
+    M, N, K = 200, 256, 320
+    w, b = 0.1 * torch.randn(N, K, device="cuda"), torch.randn(N, device="cuda")
+    x = torch.randn(M, K, device="cuda").to(BF16)
+    want = ops.linear_mxfp4(x, ops.quantize_mxfp4(w), b, gelu=True)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.linear_mxfp4(x, ops.quantize_mxfp4(w), b, gelu=True)
+    side.synchronize()
+    assert torch.equal(got, want)
+    wq = ops.quantize_mxfp4(w)
+    dy = torch.randn(M, N, device="cuda").to(BF16)
+
+    def step():
+        xq = ops.quantize_mxfp4(x)
+        return ops.linear_mxfp4(x, wq, b, gelu=True), ops.linear_mxfp4(x[:3], wq, b), G.linear_mxfp4_bwd(dy, xq, wq)[0]
+    for _ in range(2):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, c, dx = step()
+    for k in range(4):
+        x.copy_(torch.randn(M, K, device="cuda").to(BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        ea, ec, edx = step()
+        assert torch.equal(a, ea) and torch.equal(c, ec) and torch.equal(dx, edx), k
+
+
+def _grads_64(x, w, dy):
+    xv, wv, d = values(x), values(w), dy.double()
+    return d @ wv, d.t() @ xv, d.sum(0), (d.abs() @ wv.abs(), d.abs().t() @ xv.abs(), d.abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 64), (5, 33, 77), (16, 8, 40), (385, 512, 512), (200, 100, 260), (64, 65, 257), (1200, 256, 768)])
+def test_gradients_against_64_bits(M, N, K, dtype):
+    x = _x(M, K, dtype).requires_grad_(True)
+    w = (0.05 * torch.randn(N, K, device="cuda")).requires_grad_(True)
+    b = torch.randn(N, device="cuda").requires_grad_(True)
+    y = training.linear_mxfp4(x, w, b)
+    assert torch.equal(y.detach(), ops.linear_mxfp4(ops.quantize_mxfp4(x.detach()), ops.quantize_mxfp4(w.detach()), b.detach()))
+    dy = torch.randn(M, N, device="cuda").to(BF16)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ex, ew, eb, (sx, sw, sb) = _grads_64(x.detach(), w.detach(), dy)
+    assert dx.dtype == dtype and dw.dtype == F32 and db.dtype == F32
+    # dy is bf16 already and the operands are exact: products of two bf16 values are exact in fp32
+    _check(dx, ex, sx, N, 0, (UBF * (ex.abs() + N * U32 * sx)) if dtype == BF16 else 0.0)
+    _check(dw, ew, sw, M, 0)
+    _check(db, eb, sb, M, 0)
+
+
+def test_gradients_against_differences():
+    """y is linear in each quantised operand: a difference along any direction is the gradient's inner product exactly (64 bits)."""
+    M, N, K = 40, 24, 96
+    x, w = torch.randn(M, K, device="cuda"), 0.1 * torch.randn(N, K, device="cuda")
+    dy = torch.randn(M, N, device="cuda").to(BF16)
+    xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, F32)
+    loss = lambda a, c, e: ((a @ c.t() + e) * dy.double()).sum()  # noqa: E731
+    xv, wv, bv = ops.dequantize_mxfp4(xq).double(), ops.dequantize_mxfp4(wq).double(), torch.zeros(N, dtype=F64, device="cuda")
+    for grad, at in ((dx, 0), (dw, 1), (db, 2)):
+        d = torch.randn(grad.shape, dtype=F64, device="cuda")
+        args = [xv, wv, bv]
+        up, down = list(args), list(args)
+        up[at], down[at] = args[at] + d, args[at] - d
+        slope = (loss(*up) - loss(*down)) / 2
+        size = (grad.double().abs() * d.abs()).sum()
+        assert (slope - (grad.double() * d).sum()).abs() <= max(M, N) * 2.0 ** -20 * size
+
+
+def test_autograd_shapes_and_partial_gradients():
+    x = torch.randn(2, 9, 64, device="cuda", requires_grad=True)
+    w = torch.randn(32, 64, device="cuda")
+    y = training.linear_mxfp4(x, w)
+    assert y.shape == (2, 9, 32)
+    y.sum().backward()          # an expanded gradient
+    want = G.linear_mxfp4_bwd(torch.ones(18, 32, device="cuda", dtype=BF16), ops.quantize_mxfp4(x.detach().view(18, 64)), ops.quantize_mxfp4(w), F32)[0]
+    assert torch.equal(x.grad.view(18, 64), want)
+    wt = torch.randn(64, 32, device="cuda", requires_grad=True)
+    training.linear_mxfp4(x.detach(), wt.t()).float().pow(2).sum().backward()
+    assert wt.grad.shape == (64, 32) and torch.isfinite(wt.grad).all() and wt.grad.abs().sum() > 0
+    with torch.no_grad():
+        assert not training.linear_mxfp4(x, w).requires_grad
+
+
+def test_autograd_is_refused_under_capture():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    w = torch.randn(8, 64, device="cuda")
+    training.linear_mxfp4(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            training.linear_mxfp4(x, w)
+        y = training.linear_mxfp4(x.detach(), w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, training.linear_mxfp4(x.detach(), w))
