@@ -401,6 +401,27 @@ int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void 
                         int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
                         void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------
+ * (8) Orthogonalised updates (the Muon optimiser's step).  No counterpart in the reference, which trains with Adam
+ * (scripts/train_sgclip.py:232-241); for the weight matrices of the same linear layers.
+ *
+ * X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T on the shorter side: singular values
+ * go towards 1, singular vectors stay.  coefficients: host f32 [steps][3] = a, b, c of every step.  Products in two fp16 halves
+ * per operand with fp32 sums (fp32 grade).  coefficients under which values would leave fp16's range are refused.
+ * ---------------------------------------------------------------------- */
+size_t sgclip_orthogonalize_workspace_bytes(int batch, int rows, int cols);
+/* g bf16 or f32 [batch][rows][cols] (row stride ldg, batch stride batch_stride, elements; 1 <= rows, cols <= 65536) -> out bf16
+ * (ldo, out_batch_stride); out must not overlap g. */
+int sgclip_orthogonalize(const void *g_dev, int g_dtype, int64_t batch_stride, int64_t ldg, int batch, int rows, int cols,
+                         const float *coefficients, int steps, float eps, void *out_dev, int64_t out_batch_stride, int64_t ldo,
+                         void *workspace_dev, size_t workspace_bytes, void *stream);
+/* One optimiser step on `count` contiguous f32 [rows, cols] matrices, given by host tables of device pointers (read during the
+ * call only):  m = momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
+ * p = (1 - lr weight_decay) p - lr scale orthogonalize(u).  Workspace: sgclip_orthogonalize_workspace_bytes(count, ..). */
+int sgclip_muon_step(float *const *params, const float *const *grads, float *const *momenta, int count, int rows, int cols,
+                     float momentum, int nesterov, float lr, float weight_decay, float scale, const float *coefficients, int steps,
+                     float eps, void *workspace_dev, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,665 @@
+// Orthogonalised updates: Newton-Schulz iteration on batches of matrices, and the optimiser step around it.
+//
+// With X = U / (|U|_F + eps) on its short side m <= n, one step is X <- p(A) X, A = X X^T, p(t) = a + b t + c t^2: every
+// singular value s becomes s p(s^2).  A and all polynomials of it are symmetric and commute, so
+//   * every m x m product is computed on the tiles of one triangle and written to both;
+//   * several steps need X only once: M_i = p(A_i), Q <- M_i Q, A_{i+1} = M_i A_i M_i, then X <- Q X.  A block of k steps costs
+//     3 m^2 n + (4 k - 3) m^3 multiplications and additions instead of k (3 m^2 n + m^3).
+// The blocks are at most 3 steps long: squaring through A loses small singular values (the relative error of the result
+// grows from 1e-6 to 1e-5 at 3 steps and 7e-4 at 5, worst of the spectra tried, against 64 bits).
+//
+// Precision.  The first steps multiply small singular values by a each, 485 times over five steps with the usual coefficients,
+// and rounding errors with them: with bf16 products the result is off by 2 to 20 %, with fp16 by 0.2 to 3 %.  Operands are
+// therefore held as two fp16 halves, v = hi + lo (22 bits), and a product is hi hi + hi lo + lo hi with fp32 sums: fp32 grade
+// at a third of the fp16 matrix rate.  Powers of two keep the halves inside fp16's range; they are chosen on the host from
+// bounds of the polynomial over the range of singular values.
+//
+// Storage of an operand with K columns ("split rows"): row stride ceil(K / 32) * 128 bytes, per 32 columns 64 bytes of hi and
+// 64 of lo, zeros behind K.  One such piece of a row is a cache line and one stage of the product's loop.
+#include "tile_common.h"
+
+#include <math.h>
+
+namespace sgclip {
+
+typedef _Float16 f16_t;
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int OR_BATCH = 64;      // matrices per launch: their pointers travel as kernel arguments
+constexpr int OR_PARTS = 64;      // partial sums of a matrix's squared norm
+
+static __host__ __device__ inline int or_chunks(int k) { return (k + 31) / 32; }
+
+struct OrPointers {
+    void *p[OR_BATCH];
+};
+
+__device__ __forceinline__ void or_split(float v, f16_t &hi, f16_t &lo) {
+    hi = (f16_t)v;
+    lo = (f16_t)(v - (float)hi);
+}
+
+// ---------------------------------------------------------------------------
+// The products.  out[i][j] = sum_k L[i][k] R[j][k] on split rows, tile of 2 WT x 2 WT, four waves of WT x WT.
+// ---------------------------------------------------------------------------
+enum { OR_SYM = 0, OR_POLY = 1, OR_BOTH = 2, OR_OUT = 3, OR_UPDATE = 4 };
+
+struct OrGemm {
+    const unsigned char *L[2], *R;     // [2]: two products with the same R in one launch (grid z)
+    unsigned char *O[2];               // split rows [M][N], or with OR_BOTH also
+    unsigned char *OT;                 // their transpose [N][M]
+    const unsigned char *A;            // OR_POLY: A's split rows
+    long long sL, sR, sO, sOT;         // bytes from one matrix of the batch to the next
+    float alpha[2];                    // power of two from the accumulator's scale to the output's
+    float ca, cb, cc;                  // OR_POLY: out = ca I + cb A + cc (A A)
+    float decay, rate;                 // OR_UPDATE: p = decay p - rate out
+    long long ldo;                     // OR_OUT / OR_UPDATE: row stride in elements
+    int M, N, kc;                      // rows of L, rows of R, 32-column pieces of both
+    int tiles_m, tiles_n, wide;
+    OrPointers out;                    // OR_OUT: bf16, OR_UPDATE: f32 parameters
+};
+
+template <int EPI, int WT>
+__global__ __launch_bounds__(256) void or_gemm_kernel(OrGemm g) {
+    constexpr int T = 2 * WT, NT = WT / 16, OP = T * 128;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1, r = lane & 15, q = lane >> 4;
+    constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
+    const int per = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
+    const int swz = xcd_remap(blockIdx.x, gridDim.x);
+    const int b = swz / per, t = swz - b * per, z = blockIdx.z;
+    int ti, tj;
+    if (SYM) {      // t-th tile of the lower triangle, row by row
+        ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ti++;
+        while (ti * (ti + 1) / 2 > t) ti--;
+        tj = t - ti * (ti + 1) / 2;
+    } else {
+        ti = t / g.tiles_n;
+        tj = t - ti * g.tiles_n;
+    }
+    const int m0 = ti * T, n0 = tj * T;
+    const long long ld = (long long)g.kc * 128;
+    const unsigned char *L = (z ? g.L[1] : g.L[0]) + b * g.sL, *R = g.R + b * g.sR;
+
+    auto fetch = [&](int s, unsigned char *slot) {
+#pragma unroll
+        for (int p = wave; p < T / 8; p += 4) {
+            const int row = p * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+            const unsigned char *sl = L + min(m0 + row, g.M - 1) * ld + s * 128 + c * 16;
+            const unsigned char *sr = R + min(n0 + row, g.N - 1) * ld + s * 128 + c * 16;
+            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sl), LDS_PTR(slot + p * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sr), LDS_PTR(slot + OP + p * 1024), 16, 0, 0);
+        }
+    };
+    f32x4 acc[NT][NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    fetch(0, lds);
+    for (int s = 0; s < g.kc; s++) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const unsigned char *cur = lds + (s & 1) * 2 * OP;
+        if (s + 1 < g.kc) fetch(s + 1, lds + ((s + 1) & 1) * 2 * OP);
+        f16x8 lh[NT], ll[NT], rh[NT], rl[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            lh[i] = *(const f16x8 *)(cur + lds_off(wm * WT + i * 16 + r, q));
+            ll[i] = *(const f16x8 *)(cur + lds_off(wm * WT + i * 16 + r, 4 + q));
+            rh[i] = *(const f16x8 *)(cur + OP + lds_off(wn * WT + i * 16 + r, q));
+            rl[i] = *(const f16x8 *)(cur + OP + lds_off(wn * WT + i * 16 + r, 4 + q));
+        }
+        // R first: a lane's four results are four consecutive columns of one row
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
+            }
+    }
+
+    const float alpha = z ? g.alpha[1] : g.alpha[0];
+    unsigned char *O = (z ? g.O[1] : g.O[0]) + b * g.sO;
+    const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int m = m0 + wm * WT + i * 16 + r, n = n0 + wn * WT + j * 16 + q * 4;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] * alpha;
+            if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
+                if (m >= g.M || n >= g.N) continue;
+                const long long at = m * g.ldo + n;
+                if constexpr (EPI == OR_OUT) {
+                    bf16_t *o = (bf16_t *)g.out.p[b] + at;
+                    if (g.wide) {
+                        bf16x4 w;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = (bf16_t)v[e];
+                        *(bf16x4 *)o = w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < g.N) o[e] = (bf16_t)v[e];
+                    }
+                } else {
+                    float *o = (float *)g.out.p[b] + at;
+                    if (g.wide) {
+                        float4 w = *(const float4 *)o;
+                        w.x = w.x * g.decay - g.rate * v[0];
+                        w.y = w.y * g.decay - g.rate * v[1];
+                        w.z = w.z * g.decay - g.rate * v[2];
+                        w.w = w.w * g.decay - g.rate * v[3];
+                        *(float4 *)o = w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < g.N) o[e] = o[e] * g.decay - g.rate * v[e];
+                    }
+                }
+                continue;
+            }
+            if constexpr (EPI == OR_POLY) {
+                if (m < g.M && n < or_chunks(g.N) * 32) {
+                    const unsigned char *a = g.A + b * g.sL + m * ld + (n >> 5) * 128 + (n & 31) * 2;
+                    const f16x4 ah = *(const f16x4 *)a, al = *(const f16x4 *)(a + 64);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = g.cc * acc[i][j][e] + g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
+                }
+            }
+            f16x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f16_t h, l;
+                or_split(m < g.M && n + e < g.N ? v[e] : 0.f, h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            if (m < g.M && n < or_chunks(g.N) * 32) {
+                unsigned char *o = O + m * ldn + (n >> 5) * 128 + (n & 31) * 2;
+                *(f16x4 *)o = hi;
+                *(f16x4 *)(o + 64) = lo;
+            }
+            if ((EPI == OR_BOTH || ti != tj) && m < or_chunks(g.M) * 32) {
+                unsigned char *ot = (EPI == OR_BOTH ? g.OT + b * g.sOT : O) + (m >> 5) * 128 + (m & 31) * 2;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (n + e < g.N) {
+                        *(f16_t *)(ot + (n + e) * ldm) = hi[e];
+                        *(f16_t *)(ot + (n + e) * ldm + 64) = lo[e];
+                    }
+            }
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Before the products: the squared norm (and the momentum), then the two split forms of U / (|U| + eps).
+// ---------------------------------------------------------------------------
+struct OrInput {
+    OrPointers g, buf;      // buf: momentum buffers (null without a step)
+    long long ldg;
+    int rows, cols;
+    float mu;
+    int nesterov, vec;      // vec: four columns per access
+};
+
+template <typename T, bool STEP>
+__device__ __forceinline__ float or_direction(const OrInput &a, float g, float buf) {
+    if constexpr (!STEP) return g;
+    return a.nesterov ? (1.0f - a.mu) * g + a.mu * buf : buf;
+}
+
+template <typename T>
+__device__ __forceinline__ float4 or_load4(const T *p) {
+    if constexpr (sizeof(T) == 4) return *(const float4 *)p;
+    const bf16x4 v = *(const bf16x4 *)p;
+    return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+}
+
+// parts[matrix][part] = the part's sum of squares, in 64 bits: squares of large fp32 gradients pass fp32's range.  With STEP the
+// momentum buffer is updated on the way: buf = mu buf + (1 - mu) g.
+template <typename T, bool STEP>
+__global__ __launch_bounds__(256) void or_norm_kernel(OrInput a, double *__restrict__ parts) {
+    __shared__ double wsum[4];
+    const T *g = (const T *)a.g.p[blockIdx.y];
+    float *buf = (float *)a.buf.p[blockIdx.y];
+    double s = 0.0;
+    const int step = a.vec ? 4 : 1, per = a.cols / step;
+    const long long total = (long long)a.rows * per;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256 * OR_PARTS) {
+        const long long row = i / per;
+        const int col = (int)(i - row * per) * step;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), m = v;
+        if (a.vec) v = or_load4(g + row * a.ldg + col);
+        else v.x = (float)g[row * a.ldg + col];
+        if constexpr (STEP) {
+            float *bp = buf + row * a.cols + col;
+            if (a.vec) m = *(const float4 *)bp;
+            else m.x = *bp;
+            m.x = a.mu * m.x + (1.0f - a.mu) * v.x;
+            m.y = a.mu * m.y + (1.0f - a.mu) * v.y;
+            m.z = a.mu * m.z + (1.0f - a.mu) * v.z;
+            m.w = a.mu * m.w + (1.0f - a.mu) * v.w;
+            if (a.vec) *(float4 *)bp = m;
+            else *bp = m.x;
+        }
+        const float x = or_direction<T, STEP>(a, v.x, m.x), y = or_direction<T, STEP>(a, v.y, m.y);
+        const float z = or_direction<T, STEP>(a, v.z, m.z), w = or_direction<T, STEP>(a, v.w, m.w);
+        s += ((double)x * x + (double)y * y) + ((double)z * z + (double)w * w);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[blockIdx.y * OR_PARTS + blockIdx.x] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+}
+
+// 64 x 64 tiles: rows [rows][cols] and their transpose [cols][rows], both in split rows, scaled by 2^e / (norm + eps)
+template <typename T, bool STEP>
+__global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *__restrict__ parts, float scale, float eps,
+                                                       unsigned char *__restrict__ rowp, unsigned char *__restrict__ colp,
+                                                       long long srow, long long scol) {
+    __shared__ float tile[64][65];
+    __shared__ double inv_s;
+    const int tid = threadIdx.x, b = blockIdx.y;
+    if (tid < 64) {
+        double s = parts[b * OR_PARTS + tid];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (tid == 0) inv_s = (double)scale / (sqrt(s) + (double)eps);
+    }
+    __syncthreads();
+    const double inv = inv_s;
+    const T *g = (const T *)a.g.p[b];
+    const float *buf = (const float *)a.buf.p[b];
+    const int tc = (a.cols + 63) / 64;
+    const int r0 = blockIdx.x / tc * 64, c0 = blockIdx.x % tc * 64;
+    if (a.vec) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const int lr = (tid >> 4) + 16 * p, lc = (tid & 15) * 4, row = r0 + lr, col = c0 + lc;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), m = v;
+            if (row < a.rows && col < a.cols) {
+                v = or_load4(g + row * a.ldg + col);
+                if constexpr (STEP) m = *(const float4 *)(buf + (long long)row * a.cols + col);
+            }
+            tile[lr][lc] = (float)(or_direction<T, STEP>(a, v.x, m.x) * inv);
+            tile[lr][lc + 1] = (float)(or_direction<T, STEP>(a, v.y, m.y) * inv);
+            tile[lr][lc + 2] = (float)(or_direction<T, STEP>(a, v.z, m.z) * inv);
+            tile[lr][lc + 3] = (float)(or_direction<T, STEP>(a, v.w, m.w) * inv);
+        }
+    } else {
+        for (int p = 0; p < 16; p++) {
+            const int lr = (tid >> 6) + 4 * p, lc = tid & 63, row = r0 + lr, col = c0 + lc;
+            float v = 0.f;
+            if (row < a.rows && col < a.cols)
+                v = (float)(or_direction<T, STEP>(a, (float)g[row * a.ldg + col], STEP ? buf[(long long)row * a.cols + col] : 0.f) * inv);
+            tile[lr][lc] = v;
+        }
+    }
+    __syncthreads();
+    const long long ldr = (long long)or_chunks(a.cols) * 128, ldc = (long long)or_chunks(a.rows) * 128;
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const int lr = (tid >> 3) + 32 * p, l8 = (tid & 7) * 8;
+        f16x8 hi, lo;
+        if (r0 + lr < a.rows && c0 + l8 < or_chunks(a.cols) * 32) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f16_t h, l;
+                or_split(tile[lr][l8 + e], h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            unsigned char *o = rowp + b * srow + (r0 + lr) * ldr + ((c0 + l8) >> 5) * 128 + (l8 & 31) * 2;
+            *(f16x8 *)o = hi;
+            *(f16x8 *)(o + 64) = lo;
+        }
+        if (c0 + lr < a.cols && r0 + l8 < or_chunks(a.rows) * 32) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f16_t h, l;
+                or_split(tile[l8 + e][lr], h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            unsigned char *o = colp + b * scol + (c0 + lr) * ldc + ((r0 + l8) >> 5) * 128 + (l8 & 31) * 2;
+            *(f16x8 *)o = hi;
+            *(f16x8 *)(o + 64) = lo;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct OrPlan {
+    int m, n, flip;                          // short and long side; flip: the matrix has more rows than columns
+    size_t x, xt, sq, parts, total;          // bytes per matrix: X, X^T, one m x m operand; the norm's parts; all of it
+};
+
+static OrPlan or_plan(int rows, int cols) {
+    OrPlan p;
+    p.flip = rows > cols;
+    p.m = p.flip ? cols : rows;
+    p.n = p.flip ? rows : cols;
+    p.x = (size_t)p.m * or_chunks(p.n) * 128;
+    p.xt = (size_t)p.n * or_chunks(p.m) * 128;
+    p.sq = (size_t)p.m * or_chunks(p.m) * 128;
+    p.parts = OR_PARTS * sizeof(double);
+    p.total = p.x + 2 * p.xt + 5 * p.sq + p.parts;
+    return p;
+}
+
+// largest e with bound 2^e <= 2^15 (half of fp16's range is left for rounding), at most 14; false where the bound is too large
+static bool or_exponent(double bound, int &e) {
+    if (!(bound <= 4096.0)) return false;
+    e = bound <= 0 ? 14 : (int)floor(15.0 - log2(bound));
+    if (e > 14) e = 14;
+    return true;
+}
+
+struct OrStep {
+    double a, b, c;
+    int em, et, ea;     // exponents of M = p(A), of T = A M and of A' = M A M
+};
+
+constexpr int OR_STEPS = 32;
+
+// The steps' blocks and exponents from bounds over the range of singular values.
+struct OrSchedule {
+    int steps, blocks, len[OR_STEPS];
+    int ex[OR_STEPS + 1], ea0[OR_STEPS], eq[OR_STEPS];   // X at a block's start, its Gram matrix; Q after each step of its block
+    OrStep s[OR_STEPS];
+};
+
+static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSchedule &o) {
+    o.steps = steps;
+    // square matrices: blocks save nothing, single steps lose least
+    const int most = n * 4LL < m * 5LL ? 1 : 3;
+    o.blocks = (steps + most - 1) / most;
+    for (int i = 0; i < o.blocks; i++) o.len[i] = steps / o.blocks + (i < steps % o.blocks);
+    double top = 1.0, qb = 1.0;     // bounds of the singular values (1 after the normalisation) and of Q
+    for (int k = 0, blk = 0, in = 0; k < steps; k++) {
+        const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+        o.s[k].a = a;
+        o.s[k].b = b;
+        o.s[k].c = c;
+        if (in == 0 && (!or_exponent(top, o.ex[blk]) || !or_exponent(top * top, o.ea0[blk]))) return false;
+        double pm = 0, tm = 0, next = 0;
+        for (int i = 0; i <= 1024; i++) {
+            const double s = top * i / 1024, t = s * s, p = fabs(a + b * t + c * t * t);
+            pm = fmax(pm, p);
+            tm = fmax(tm, t * p);
+            next = fmax(next, s * p);
+        }
+        if (!(pm == pm) || !or_exponent(pm, o.s[k].em) || !or_exponent(tm, o.s[k].et) || !or_exponent(next * next, o.s[k].ea)) return false;
+        qb = in == 0 ? pm : qb * pm;
+        if (!or_exponent(qb, o.eq[k])) return false;
+        top = next;
+        if (++in == o.len[blk]) {
+            in = 0;
+            blk++;
+        }
+    }
+    return or_exponent(top, o.ex[o.blocks]);
+}
+
+template <int EPI>
+static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t stream) {
+    OrGemm g = gin;
+    constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
+    auto tiles = [&](int T) {
+        g.tiles_m = ceil_div(g.M, T);
+        g.tiles_n = ceil_div(g.N, T);
+        return (long long)batch * (SYM ? (long long)g.tiles_m * (g.tiles_m + 1) / 2 : (long long)g.tiles_m * g.tiles_n);
+    };
+    // 128 x 128 tiles where they fill the chip, 64 x 64 below that
+    long long blocks = tiles(128);
+    if (blocks * products * 4 * 256 > 0xffffffffLL) {   // 64 x 64 tiles at most; a launch counts its threads in 32 bits
+        set_error("sgclip_orthogonalize: %d matrices of %d x %d are more than one launch holds", batch, g.M, g.N);
+        return SGCLIP_EINVAL;
+    }
+    if (blocks * products >= device_cus()) {
+        if (!lds_attr((const void *)or_gemm_kernel<EPI, 64>, 4 * 128 * 128)) return SGCLIP_ELAUNCH;
+        or_gemm_kernel<EPI, 64><<<dim3((unsigned)blocks, 1, products), 256, 4 * 128 * 128, stream>>>(g);
+    } else {
+        blocks = tiles(64);
+        or_gemm_kernel<EPI, 32><<<dim3((unsigned)blocks, 1, products), 256, 4 * 64 * 128, stream>>>(g);
+    }
+    return launch_check("sgclip_orthogonalize");
+}
+
+static inline float or_pow2(int e) { return ldexpf(1.0f, e); }
+
+// One launch group of up to OR_BATCH matrices.  in: gradients (and momentum buffers); out: bf16 results or parameters.
+template <typename T, bool STEP>
+static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
+                  unsigned char *ws, hipStream_t stream) {
+    const OrPlan p = or_plan(in.rows, in.cols);
+    unsigned char *X = ws, *XT = X + p.x * batch, *XT2 = XT + p.xt * batch, *A = XT2 + p.xt * batch, *M = A + p.sq * batch, *Tm = M + p.sq * batch,
+                  *Q = Tm + p.sq * batch, *Q2 = Q + p.sq * batch;
+    double *parts = (double *)(Q2 + p.sq * batch);
+    or_norm_kernel<T, STEP><<<dim3(OR_PARTS, batch), 256, 0, stream>>>(in, parts);
+    const int tiles = ceil_div(in.rows, 64) * ceil_div(in.cols, 64);
+    or_split_kernel<T, STEP><<<dim3(tiles, batch), 256, 0, stream>>>(in, parts, or_pow2(sch.ex[0]), eps, p.flip ? XT : X, p.flip ? X : XT,
+                                                                     p.flip ? p.xt : p.x, p.flip ? p.x : p.xt);
+    int rc = launch_check("sgclip_orthogonalize");
+    const int km = or_chunks(p.m), kn = or_chunks(p.n);
+    for (int blk = 0, k = 0; blk < sch.blocks && rc == SGCLIP_OK; blk++) {
+        int ea = sch.ea0[blk], eq = 0;
+        OrGemm g{};
+        g.M = g.N = p.m;
+        g.L[0] = g.R = X;
+        g.O[0] = A;
+        g.sL = g.sR = (long long)p.x;
+        g.sO = (long long)p.sq;
+        g.kc = kn;
+        g.alpha[0] = or_pow2(ea - 2 * sch.ex[blk]);
+        rc = or_launch<OR_SYM>(g, batch, 1, stream);
+        g.sL = g.sR = (long long)p.sq;
+        g.kc = km;
+        for (int i = 0; i < sch.len[blk] && rc == SGCLIP_OK; i++, k++) {
+            const OrStep &s = sch.s[k];
+            const bool last = i + 1 == sch.len[blk];
+            // M = a I + b A + c A A (into Q on the block's first step)
+            g.L[0] = g.R = g.A = A;
+            unsigned char *Mi = i == 0 ? Q : M;
+            g.O[0] = Mi;
+            g.ca = (float)ldexp(s.a, s.em);
+            g.cb = (float)ldexp(s.b, s.em - ea);
+            g.cc = (float)ldexp(s.c, s.em - 2 * ea);
+            if ((rc = or_launch<OR_POLY>(g, batch, 1, stream)) != SGCLIP_OK) break;
+            if (i == 0) eq = s.em;
+            // T = A M and Q = Q M, whichever are needed
+            int np = 0;
+            g.R = Mi;
+            if (!last) {
+                g.L[np] = A;
+                g.O[np] = Tm;
+                g.alpha[np++] = or_pow2(s.et - ea - s.em);
+            }
+            if (i > 0) {
+                g.L[np] = Q;
+                g.O[np] = Q2;
+                g.alpha[np++] = or_pow2(sch.eq[k] - eq - s.em);
+                eq = sch.eq[k];
+            }
+            if (np && (rc = or_launch<OR_SYM>(g, batch, np, stream)) != SGCLIP_OK) break;
+            if (i > 0) {
+                unsigned char *swap = Q;
+                Q = Q2;
+                Q2 = swap;
+            }
+            if (!last) {     // A = T M
+                g.L[0] = Tm;
+                g.O[0] = A;
+                g.alpha[0] = or_pow2(s.ea - s.et - s.em);
+                ea = s.ea;
+                if ((rc = or_launch<OR_SYM>(g, batch, 1, stream)) != SGCLIP_OK) break;
+            }
+        }
+        if (rc != SGCLIP_OK) break;
+        // X = Q X: rows of Q against rows of X^T; the last one goes out in the matrix's own orientation
+        g.L[0] = Q;
+        g.R = XT;
+        g.sL = (long long)p.sq;
+        g.sR = (long long)p.xt;
+        g.M = p.m;
+        g.N = p.n;
+        if (blk + 1 < sch.blocks) {
+            g.O[0] = X;          // read by nothing in this product; X^T is, so its successor goes to the other buffer
+            g.sO = (long long)p.x;
+            g.OT = XT2;
+            g.sOT = (long long)p.xt;
+            g.alpha[0] = or_pow2(sch.ex[blk + 1] - eq - sch.ex[blk]);
+            rc = or_launch<OR_BOTH>(g, batch, 1, stream);
+            unsigned char *swap = XT;
+            XT = XT2;
+            XT2 = swap;
+        } else {
+            if (p.flip) {
+                g.L[0] = XT;
+                g.R = Q;
+                g.sL = (long long)p.xt;
+                g.sR = (long long)p.sq;
+                g.M = p.n;
+                g.N = p.m;
+            }
+            g.out = out;
+            g.ldo = ldo;
+            g.alpha[0] = or_pow2(-eq - sch.ex[blk]);
+            g.decay = decay;
+            g.rate = rate;
+            g.wide = g.N % 4 == 0 && ldo % 4 == 0;
+            for (int i = 0; i < batch; i++) g.wide = g.wide && ((uintptr_t)out.p[i] & 15) == 0;
+            rc = STEP ? or_launch<OR_UPDATE>(g, batch, 1, stream) : or_launch<OR_OUT>(g, batch, 1, stream);
+        }
+    }
+    return rc;
+}
+
+}  // namespace sgclip
+
+using namespace sgclip;
+
+static bool or_args_ok(const char *who, int rows, int cols, const float *coefficients, int steps, float eps, OrSchedule &sch) {
+    if (rows <= 0 || cols <= 0 || rows > 65536 || cols > 65536) {
+        set_error("%s: bad shape rows=%d cols=%d (1 to 65536)", who, rows, cols);
+        return false;
+    }
+    if (!coefficients || steps < 1 || steps > OR_STEPS || !(eps >= 0.f)) {
+        set_error("%s: bad steps=%d (1 to %d), coefficients or eps=%g", who, steps, OR_STEPS, (double)eps);
+        return false;
+    }
+    const OrPlan p = or_plan(rows, cols);
+    if (!or_schedule(coefficients, steps, p.m, p.n, sch)) {
+        set_error("%s: with these coefficients singular values or a step's polynomial grow beyond fp16's range", who);
+        return false;
+    }
+    return true;
+}
+
+static bool or_workspace_ok(const char *who, const void *ws, size_t have, int batch, int rows, int cols) {
+    const size_t need = sgclip_orthogonalize_workspace_bytes(batch, rows, cols);
+    if (!ws || have < need || ((uintptr_t)ws & 15)) {
+        set_error("%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, ws ? have : (size_t)0, need);
+        return false;
+    }
+    return true;
+}
+
+extern "C" {
+
+size_t sgclip_orthogonalize_workspace_bytes(int batch, int rows, int cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    return or_plan(rows, cols).total * (size_t)(batch < OR_BATCH ? batch : OR_BATCH);
+}
+
+int sgclip_orthogonalize(const void *g_dev, int g_dtype, int64_t batch_stride, int64_t ldg, int batch, int rows, int cols,
+                         const float *coefficients, int steps, float eps, void *out_dev, int64_t out_batch_stride, int64_t ldo,
+                         void *workspace_dev, size_t workspace_bytes, void *stream) {
+    const char *who = "sgclip_orthogonalize";
+    if (batch == 0) return SGCLIP_OK;
+    OrSchedule sch;
+    if (!or_args_ok(who, rows, cols, coefficients, steps, eps, sch)) return SGCLIP_EINVAL;
+    if (batch < 0 || !g_dev || !out_dev || ldg < cols || ldo < cols || (g_dtype != SGCLIP_DTYPE_F32 && g_dtype != SGCLIP_DTYPE_BF16) ||
+        (batch > 1 && out_batch_stride < (int64_t)(rows - 1) * ldo + cols)) {
+        set_error("%s: bad matrices (batch %d, dtype %d, row strides %lld and %lld, output batch stride %lld, cols %d)", who, batch, g_dtype,
+                  (long long)ldg, (long long)ldo, (long long)out_batch_stride, cols);
+        return SGCLIP_EINVAL;
+    }
+    if (!or_workspace_ok(who, workspace_dev, workspace_bytes, batch, rows, cols)) return SGCLIP_ENOSPC;
+    const size_t size = g_dtype == SGCLIP_DTYPE_F32 ? 4 : 2;
+    int rc = SGCLIP_OK;
+    for (int b0 = 0; b0 < batch && rc == SGCLIP_OK; b0 += OR_BATCH) {
+        const int n = batch - b0 < OR_BATCH ? batch - b0 : OR_BATCH;
+        OrInput in{};
+        OrPointers out{};
+        in.ldg = ldg;
+        in.rows = rows;
+        in.cols = cols;
+        in.vec = cols % 4 == 0 && ldg % 4 == 0;
+        for (int i = 0; i < n; i++) {
+            in.g.p[i] = (char *)g_dev + (b0 + i) * batch_stride * (int64_t)size;
+            out.p[i] = (char *)out_dev + (b0 + i) * out_batch_stride * 2;
+            in.vec = in.vec && ((uintptr_t)in.g.p[i] & 15) == 0;
+        }
+        rc = g_dtype == SGCLIP_DTYPE_F32
+                 ? or_run<float, false>(in, out, ldo, n, sch, eps, 1.f, 0.f, (unsigned char *)workspace_dev, (hipStream_t)stream)
+                 : or_run<bf16_t, false>(in, out, ldo, n, sch, eps, 1.f, 0.f, (unsigned char *)workspace_dev, (hipStream_t)stream);
+    }
+    return rc;
+}
+
+int sgclip_muon_step(float *const *params, const float *const *grads, float *const *momenta, int count, int rows, int cols, float momentum,
+                     int nesterov, float lr, float weight_decay, float scale, const float *coefficients, int steps, float eps,
+                     void *workspace_dev, size_t workspace_bytes, void *stream) {
+    const char *who = "sgclip_muon_step";
+    if (count == 0) return SGCLIP_OK;
+    OrSchedule sch;
+    if (!or_args_ok(who, rows, cols, coefficients, steps, eps, sch)) return SGCLIP_EINVAL;
+    if (count < 0 || !params || !grads || !momenta) {
+        set_error("%s: bad count %d or pointer tables", who, count);
+        return SGCLIP_EINVAL;
+    }
+    for (int i = 0; i < count; i++)
+        if (!params[i] || !grads[i] || !momenta[i]) {
+            set_error("%s: matrix %d has a null parameter, gradient or momentum", who, i);
+            return SGCLIP_EINVAL;
+        }
+    if (!or_workspace_ok(who, workspace_dev, workspace_bytes, count, rows, cols)) return SGCLIP_ENOSPC;
+    int rc = SGCLIP_OK;
+    for (int b0 = 0; b0 < count && rc == SGCLIP_OK; b0 += OR_BATCH) {
+        const int n = count - b0 < OR_BATCH ? count - b0 : OR_BATCH;
+        OrInput in{};
+        OrPointers out{};
+        in.ldg = cols;
+        in.rows = rows;
+        in.cols = cols;
+        in.mu = momentum;
+        in.nesterov = nesterov;
+        in.vec = cols % 4 == 0;
+        for (int i = 0; i < n; i++) {
+            in.g.p[i] = (void *)grads[b0 + i];
+            in.buf.p[i] = momenta[b0 + i];
+            out.p[i] = params[b0 + i];
+            in.vec = in.vec && (((uintptr_t)in.g.p[i] | (uintptr_t)in.buf.p[i]) & 15) == 0;
+        }
+        rc = or_run<float, true>(in, out, cols, n, sch, eps, 1.0f - lr * weight_decay, lr * scale, (unsigned char *)workspace_dev,
+                                 (hipStream_t)stream);
+    }
+    return rc;
+}
+
+}  // extern "C"

@@ -5,13 +5,15 @@ train step's backward pass is one of the calls below (or `ops.gemm_bf16`).
 """
 from __future__ import annotations
 
+import ctypes as C
+import functools
 import os
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .ops import Mxfp4, _ptr, _same_device, _stream, dequantize_mxfp4, gemm_bf16
+from .ops import Mxfp4, _apart, _ptr, _same_device, _stream, dequantize_mxfp4, gemm_bf16
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -287,3 +289,80 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
             gemm_bf16(dyp, w_t, dx, _lib.EPI_BIAS_BF16, bias=torch.zeros(K, dtype=F32, device=dev))
     dw = linear_wgrad(dyb, dequantize_mxfp4(xq)) if need_dw else None
     return dx, dw, db
+
+
+# -- orthogonalised updates --------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # a, b, c: steepest at 0 with singular values kept within about 0.7 .. 1.2
+
+
+@functools.lru_cache(maxsize=64)
+def _coefficient_table(coefficients: tuple, steps: int):
+    """C array f32 [steps][3] of one triple for all steps or of a triple per step."""
+    rows = (coefficients,) * steps if not isinstance(coefficients[0], tuple) else coefficients
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError(f"coefficients: one (a, b, c) or {steps} of them, got {coefficients}")
+    return (C.c_float * (3 * steps))(*(float(v) for r in rows for v in r))
+
+
+def _coefficients(coefficients, steps: int):
+    if steps < 1:
+        raise ValueError(f"{steps} Newton-Schulz steps")
+    first = coefficients[0]
+    key = tuple(tuple(float(v) for v in r) for r in coefficients) if isinstance(first, (tuple, list)) else tuple(float(v) for v in coefficients)
+    return _coefficient_table(key, steps)
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of each matrix of g (bf16 / f32 [rows, cols] or [batch, rows, cols], rows contiguous):
+    X = g / (|g| + eps), `steps` times X <- a X + (b A + c A^2) X with A = X X^T on the shorter side; bf16, shaped as g.
+    coefficients: (a, b, c), or one such triple per step.  fp32 grade inside, one rounding at the end."""
+    if g.dim() not in (2, 3) or g.dtype not in (BF16, F32) or g.device.type != "cuda":
+        raise ValueError(f"orthogonalize: expected bf16 or f32 [rows, cols] or [batch, rows, cols] on the GPU, got {g.dtype} {tuple(g.shape)} on {g.device}")
+    batch, (rows, cols) = (g.shape[0] if g.dim() == 3 else 1), g.shape[-2:]
+    table = _coefficients(coefficients, steps)
+    if out is None:
+        out = torch.empty(g.shape, dtype=BF16, device=g.device)
+    if g.numel() == 0:
+        return out
+    if out.shape != g.shape or out.dtype != BF16:
+        raise ValueError(f"orthogonalize: out must be bf16 {tuple(g.shape)}, got {out.dtype} {tuple(out.shape)}")
+    for name, t in (("g", g), ("out", out)):
+        if (cols > 1 and t.stride(-1) != 1) or (rows > 1 and t.stride(-2) < cols):
+            raise ValueError(f"orthogonalize: rows of {name} must be contiguous and apart, got strides {t.stride()}")
+    _same_device(g, out)
+    _apart("orthogonalize", out, g)
+    ld = [t.stride(-2) if rows > 1 else cols for t in (g, out)]
+    bs = [t.stride(0) if batch > 1 else rows * cols for t in (g, out)]
+    lib = _lib.load()
+    need = lib.sgclip_orthogonalize_workspace_bytes(batch, rows, cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=g.device)
+    _lib.check(lib.sgclip_orthogonalize(g.data_ptr(), _dtype_code(g), bs[0], ld[0], batch, rows, cols, table, steps, eps, out.data_ptr(), bs[1],
+                                        ld[1], ws.data_ptr(), need, _stream(g)))
+    return out
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], lr: float, momentum: float = 0.95,
+              nesterov: bool = True, weight_decay: float = 0.0, scale: float = 1.0, steps: int = 5, coefficients=NEWTON_SCHULZ,
+              eps: float = 1e-7):
+    """One orthogonalised-momentum step on matrices of one shape (contiguous f32 [rows, cols] each), in place:
+    m = momentum m + (1 - momentum) g; u = (1 - momentum) g + momentum m (nesterov) or m;
+    p = (1 - lr weight_decay) p - lr scale orthogonalize(u).  The matrices of a call share its launches."""
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    if not params:
+        return
+    shape, dev = params[0].shape, params[0].device
+    if len(shape) != 2 or dev.type != "cuda":
+        raise ValueError(f"muon_step: expected matrices on the GPU, got {tuple(shape)} on {dev}")
+    for t in (*params, *grads, *momenta):
+        if t.dtype != F32 or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"muon_step: every tensor must be contiguous f32 {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if len({t.data_ptr() for t in (*params, *momenta)}) != 2 * len(params):
+        raise ValueError("muon_step: a parameter or momentum occurs twice")
+    table = _coefficients(coefficients, steps)
+    lib, n = _lib.load(), len(params)
+    tables = [(C.c_void_p * n)(*(t.data_ptr() for t in ts)) for ts in (params, grads, momenta)]
+    need = lib.sgclip_orthogonalize_workspace_bytes(n, *shape)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.check(lib.sgclip_muon_step(*tables, n, shape[0], shape[1], momentum, 1 if nesterov else 0, lr, weight_decay, scale, table, steps, eps,
+                                    ws.data_ptr(), need, _stream(params[0])))

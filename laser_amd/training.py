@@ -584,6 +584,69 @@ class Adam:
             torch.autograd.graph.increment_version(p)   # the towers rebuild their bf16 copies when this changes
 
 
+def split_for_muon(named_parameters):
+    """(matrices, rest): the 2-D weights of the encoder layers, whose update `Muon` orthogonalises, and everything else
+    (embeddings, projections, norms, biases, the logit scale), which stays with `Adam`."""
+    matrices, rest = [], []
+    for name, p in named_parameters:
+        (matrices if p.dim() == 2 and ".encoder.layers." in name else rest).append(p)
+    return matrices, rest
+
+
+class Muon:
+    """Momentum whose direction is orthogonalised (Newton-Schulz) before it is applied, for weight matrices:
+    m = momentum m + (1 - momentum) g, u = Nesterov's or m itself, p = (1 - lr weight_decay) p - lr s orthogonalize(u).
+    adjust "rms": s = 0.2 sqrt(max(rows, cols)), an update of the size Adam's has, so that Adam's learning rates carry over;
+    "spectral": s = sqrt(max(1, rows / cols)).
+
+    Matrices of one shape take their launches together; their momenta lie in one buffer per shape (`momentum`, in the order
+    `groups` lists).  Parameters without a gradient are left as they are.  With `FlatParameters` the matrices are the
+    parameters themselves (their `.grad` are views of the flat buffer):
+
+        matrices, rest = split_for_muon(model.named_parameters())
+        opts = Muon(matrices, lr=2e-4), Adam(rest, lr=1e-5)
+    """
+
+    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+                 coefficients=G.NEWTON_SCHULZ, eps: float = 1e-7, adjust: str = "rms"):
+        self.params = [p for p in params if p.requires_grad]
+        if adjust not in ("rms", "spectral"):
+            raise ValueError(f"Muon: adjust {adjust!r}, neither 'rms' nor 'spectral'")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("Muon: a parameter occurs twice")
+        for p in self.params:
+            if p.dim() != 2 or p.dtype != F32 or not p.is_contiguous() or p.numel() == 0:
+                raise ValueError(f"Muon: contiguous f32 matrices, got {p.dtype} {tuple(p.shape)}")
+        self.lr, self.beta, self.nesterov, self.weight_decay = lr, momentum, nesterov, weight_decay
+        self.steps, self.coefficients, self.eps, self.adjust = steps, coefficients, eps, adjust
+        by_shape: Dict[tuple, List[nn.Parameter]] = {}
+        for p in self.params:
+            by_shape.setdefault((p.device, tuple(p.shape)), []).append(p)
+        self.groups = list(by_shape.values())
+        self.momentum = [torch.zeros((len(g),) + tuple(g[0].shape), dtype=F32, device=g[0].device) for g in self.groups]
+
+    def zero_grad(self, set_to_none: bool = True):
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    @torch.no_grad()
+    def step(self):
+        for group, buf in zip(self.groups, self.momentum):
+            at = [i for i, p in enumerate(group) if p.grad is not None]
+            if not at:
+                continue
+            rows, cols = group[0].shape
+            scale = 0.2 * max(rows, cols) ** 0.5 if self.adjust == "rms" else max(1.0, rows / cols) ** 0.5
+            params = [group[i] for i in at]
+            G.muon_step([p.data for p in params], [p.grad.to(F32).contiguous() for p in params], [buf[i] for i in at], self.lr, self.beta,
+                        self.nesterov, self.weight_decay, scale, self.steps, self.coefficients, self.eps)
+            for p in params:
+                torch.autograd.graph.increment_version(p)   # the towers rebuild their bf16 copies when this changes
+
+
 def allreduce_gradients(params, group=None, bucket_bytes: int = 256 << 20):
     """Average `.grad` over the ranks of `group` (RCCL on GPUs): gradients are packed into flat fp32
     buckets of about `bucket_bytes` so that each all-reduce is large enough to run at link bandwidth.
