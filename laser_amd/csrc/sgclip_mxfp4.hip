@@ -305,6 +305,207 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
         for (int j = 0; j < NT; j++) mx_store4<EPI>(g, acc[i][j], mrow + i * 16 + r, nrow + j * 16 + q * 4);
 }
 
+// ---------------------------------------------------------------------------
+// Many tiles: persistent workgroups, 256 x 256 tiles, eight waves of 128 rows x 64 columns.
+// The stages of a workgroup's tiles form one stream through two LDS slots; a stage is two 128-deep sub-steps whose fragments are
+// double-buffered in registers, with one barrier between them: there every wave holds all of stage g, stage g + 1 has landed,
+// and the DMA of stage g + 2 (of the next tile, if need be) starts into the slot just freed.  A tile's results leave through
+// a staging area of their own, so the next tile's operands arrive meanwhile; the barrier after them waits for the
+// fetches only (they are older than the stores, and the counter retires in order).
+// ---------------------------------------------------------------------------
+constexpr int MXP_OP = 256 * 128, MXP_SLOT = 2 * MXP_OP + 4096, MXP_BIAS = 2 * MXP_SLOT, MXP_STAGE = MXP_BIAS + 4096, MXP_ROW = 144;
+constexpr int MXP_LDS = MXP_STAGE + 8 * 16 * MXP_ROW;
+static_assert(MXP_LDS <= 160 * 1024, "LDS of a CU");
+
+struct MxFrags {
+    i32x4 x[8], w[4];
+    unsigned sx[2], sw;
+};
+
+__device__ __forceinline__ void mxp_read(MxFrags &f, const unsigned char *x, const unsigned char *w, const unsigned char *sx,
+                                         const unsigned char *sw) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f.x[i] = *(const i32x4 *)(x + i * 2048);
+#pragma unroll
+    for (int j = 0; j < 4; j++) f.w[j] = *(const i32x4 *)(w + j * 2048);
+    f.sx[0] = *(const unsigned *)sx;
+    f.sx[1] = *(const unsigned *)(sx + 512);
+    f.sw = *(const unsigned *)sw;
+}
+
+__device__ __forceinline__ void mxp_multiply(f32x4 (&acc)[8][4], const MxFrags &f) {
+    static_for<0, 8>([&](auto ic) {
+        static_for<0, 4>([&](auto jc) {
+            constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(f.w[j]), mx_operand(f.x[i]), acc[i][j], 4, 4, j, (int)f.sw,
+                                                                         i % 4, (int)f.sx[i / 4]);
+        });
+    });
+#pragma unroll
+    for (int p = 0; p < 15; p++) {
+        __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+    }
+}
+
+// vector memory stores of a wave for a whole tile, all younger than its last fetch
+template <int EPI>
+constexpr int mxp_stores() {
+    return EPI == MX_RESID ? 32 : 16;
+}
+
+template <int EPI>
+__device__ __forceinline__ void mxp_epilogue(const MxGemm &g, f32x4 (&acc)[8][4], const unsigned char *bias, unsigned char *region, int mw, int nw,
+                                             int lane) {
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (EPI == MX_RESID) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int jj = 0; jj < 2; jj++) {
+                    const int j = half * 2 + jj;
+                    f32x4 v = acc[i][j];
+                    if (g.bias) v += *(const f32x4 *)(bias + (j * 16 + q * 4) * 4);
+                    *(f32x4 *)(region + r * MXP_ROW + jj * 64 + q * 16) = v;
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int row = (lane >> 3) + 8 * h, m = mw + i * 16 + row, n = nw + half * 32 + (lane & 7) * 4;
+                    const f32x4 v = *(const f32x4 *)(region + row * MXP_ROW + (lane & 7) * 16);
+                    if (m < g.M && n < g.N) {
+                        const f32x4 rv = *(const f32x4 *)(g.resid + m * g.ldr + n);
+                        *(f32x4 *)((float *)g.out + m * g.ldo + n) = rv + v;
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                f32x4 v = acc[i][j];
+                if (g.bias) v += *(const f32x4 *)(bias + (j * 16 + q * 4) * 4);
+                bf16x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v[e]) : v[e]);
+                *(bf16x4 *)(region + r * MXP_ROW + j * 32 + q * 8) = o;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = (lane >> 3) + 8 * h, m = mw + i * 16 + row, n = nw + (lane & 7) * 8;
+                const bf16x8 v = *(const bf16x8 *)(region + row * MXP_ROW + (lane & 7) * 16);
+                if (m < g.M && n < g.N) {
+                    bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
+                    if (n + 8 <= g.N) *(bf16x8 *)o = v;
+                    else *(bf16x4 *)o = (bf16x4){v[0], v[1], v[2], v[3]};
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+}
+
+template <int EPI>
+__global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, int tiles_n) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 2, wn = wave & 3, r = lane & 15, q = lane >> 4;
+    const int ns = (int)(g.kp / MX_K);
+    const long long ld = g.kp / 2, rbs = g.kp * 2;    // bytes of a row's codes, of 64 rows' scales
+    const unsigned lds0 = (unsigned)(uintptr_t)LDS_PTR(lds);
+
+    // the fetch stream: next stage to fetch, of which tile
+    const int prow = wave * 8 + (lane >> 3);
+    const unsigned chunk = (unsigned)(((lane & 7) ^ ((prow >> 1) & 7)) * 16), voff = (unsigned)(prow * ld) + chunk, step = (unsigned)(64 * ld);
+    const unsigned sc_lane = (lane & 31) * 16, sc_voff = (unsigned)(((wave & 1) * 2 + (lane >> 5)) * rbs) + sc_lane;
+    const unsigned char *xb, *wb, *sb;
+    unsigned maxx, maxw, maxs;
+    int ft = blockIdx.x, fs = 0, fbias = 0, fn0 = 0, fslot = 0;
+    auto origin = [&](int t, int &m0, int &n0) {
+        const int swz = xcd_remap(t, ntiles), tm = swz / tiles_n;
+        m0 = tm * 256;
+        n0 = (swz - tm * tiles_n) * 256;
+    };
+    auto aim = [&]() {
+        int m0, n0;
+        origin(ft, m0, n0);
+        fn0 = n0;
+        xb = g.xc + m0 * ld;
+        wb = g.wc + n0 * ld;
+        maxx = (unsigned)(min(g.M - 1 - m0, 255) * ld) + chunk;
+        maxw = (unsigned)(min(g.N - 1 - n0, 255) * ld) + chunk;
+        const int rb0 = (wave < 2 ? m0 : n0) >> 6, last = ((wave < 2 ? g.M : g.N) - 1) >> 6;
+        sb = (wave < 2 ? g.xs : g.ws) + rb0 * rbs;
+        maxs = (unsigned)(min(last - rb0, 3) * rbs) + sc_lane;
+    };
+    auto fetch = [&]() {
+        if (ft >= ntiles) return;
+        const unsigned slot = lds0 + fslot * MXP_SLOT;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            p64_dma16(xb, voff, p * step, maxx, slot + (wave + 8 * p) * 1024);
+            p64_dma16(wb, voff, p * step, maxw, slot + MXP_OP + (wave + 8 * p) * 1024);
+        }
+        if (wave < 4) p64_dma16(sb, sc_voff, 0, maxs, slot + 2 * MXP_OP + wave * 1024);
+        else if (wave == 4 && fs == 0 && g.bias)
+            p64_dma16((const unsigned char *)(g.bias + fn0), lane * 16, 0, (unsigned)(min(g.N - fn0, 256) * 4 - 16), lds0 + MXP_BIAS + fbias * 1024);
+        xb += 128;
+        wb += 128;
+        sb += 512;
+        fslot ^= 1;
+        if (++fs == ns) {
+            fs = 0;
+            fbias = (fbias + 1) & 3;
+            ft += gridDim.x;
+            if (ft < ntiles) aim();
+        }
+    };
+    const int x0 = lds_off(wm * 128 + r, q), x1 = lds_off(wm * 128 + r, 4 + q);
+    const int w0 = MXP_OP + lds_off(wn * 64 + r, q), w1 = MXP_OP + lds_off(wn * 64 + r, 4 + q);
+    const int sx0 = 2 * MXP_OP + wm * 1024 + q * 64 + r * 4, sw0 = 2 * MXP_OP + 2048 + wn * 512 + q * 64 + r * 4;   // sub-step 1: + 256
+
+    aim();
+    fetch();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch();
+    f32x4 acc[8][4];
+    MxFrags f0, f1;
+    mxp_read(f0, lds + x0, lds + w0, lds + sx0, lds + sw0);
+    int slot = 0, bias = 0;   // bias: of four, since the fetch of a tile two further on may run before this tile's epilogue
+    bool stored = false;      // the last tile's stores were all issued and may still be on their way
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < ns; s++) {
+            const unsigned char *cur = lds + slot * MXP_SLOT, *nxt = lds + (slot ^ 1) * MXP_SLOT;
+            mxp_read(f1, cur + x1, cur + w1, cur + sx0 + 256, cur + sw0 + 256);
+            mxp_multiply(acc, f0);
+            if (s == 0 && stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(mxp_stores<EPI>()) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            fetch();
+            // behind the workgroup's last stage this reads what the slot held before: not used
+            mxp_read(f0, nxt + x0, nxt + w0, nxt + sx0, nxt + sw0);
+            mxp_multiply(acc, f1);
+            slot ^= 1;
+        }
+        int m0, n0;
+        origin(t, m0, n0);
+        mxp_epilogue<EPI>(g, acc, lds + MXP_BIAS + bias * 1024 + wn * 256, lds + MXP_STAGE + wave * (16 * MXP_ROW), m0 + wm * 128, n0 + wn * 64, lane);
+        bias = (bias + 1) & 3;
+        stored = m0 + 256 <= g.M && n0 + 256 <= g.N;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 // Up to 16 rows of x, quantised on the way in: a workgroup takes 16 columns of y, its eight waves 128-deep slices of K in turn,
 // and joins their sums through LDS.  A lane holds one block of 32 of one row, so the block's maximum needs no exchange.
 // Bound by the weights' bytes (and, below about a megabyte of them, by the launch).
@@ -388,6 +589,12 @@ static int mx_launch_quantize(const T *x, long long ldx, int rows, int cols, uns
 
 template <int EPI>
 static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
+    const long long huge = (((long long)g.M + 255) / 256) * (((long long)g.N + 255) / 256);
+    if (g.wide && huge >= device_cus() && huge < (1 << 24)) {
+        if (!lds_attr((const void *)mx_pipe_kernel<EPI>, MXP_LDS)) return SGCLIP_ELAUNCH;
+        mx_pipe_kernel<EPI><<<dim3((unsigned)device_cus()), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
+        return SGCLIP_OK;
+    }
     // 128 x 128 tiles where they fill the chip, 64 x 64 below that
     const long long big = (((long long)g.M + 127) / 128) * (((long long)g.N + 127) / 128);
     if (!mx_grid_ok("sgclip_mxfp4_gemm", big, 256)) return SGCLIP_EINVAL;

@@ -19,6 +19,7 @@
 #include "tile_common.h"
 
 #include <math.h>
+#include <stdlib.h>
 
 namespace sgclip {
 
@@ -60,12 +61,95 @@ struct OrGemm {
     OrPointers out;                    // OR_OUT: bf16, OR_UPDATE: f32 parameters
 };
 
-template <int EPI, int WT>
-__global__ __launch_bounds__(256) void or_gemm_kernel(OrGemm g) {
-    constexpr int T = 2 * WT, NT = WT / 16, OP = T * 128;
+// A wave's results in split rows: per 16 rows through the wave's own LDS, so that the stores are 16 bytes of whole pieces.
+// Items of a row in memory order: per 32 columns four 16-byte units of hi, then four of lo.
+__device__ __forceinline__ long long or_unit(int col) { return (long long)(col >> 5) * 128 + (col & 31) * 2; }
+
+// v: the wave's results for 16 rows (m0 ..) x 16 SN columns (n0 ..); columns at or behind N are zeros in the padding.
+template <int SN>
+__device__ __forceinline__ void or_store_rows(const f32x4 (&v)[SN], unsigned char *region, unsigned char *O, long long ld, int m0, int n0, int M,
+                                              int N, int lane) {
+    constexpr int RS = SN * 64 + 16;     // bytes of a staged row: 16 SN columns x 4, and 16 against bank conflicts
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < SN; j++) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f16_t h, l;
+            or_split(n0 + j * 16 + q * 4 + e < N ? v[j][e] : 0.f, h, l);
+            hi[e] = h;
+            lo[e] = l;
+        }
+        unsigned char *p = region + r * RS + (j * 2 + (q >> 1)) * 32 + (q & 1) * 8;
+        *(f16x4 *)p = hi;
+        *(f16x4 *)(p + 16) = lo;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int npad = or_chunks(N) * 32;
+#pragma unroll
+    for (int it0 = 0; it0 < 16 * SN * 4; it0 += 64) {
+        const int it = it0 + lane, row = it / (SN * 4), w = it - row * (SN * 4);     // w: unit of 8 columns, hi / lo
+        int u, half;
+        if (SN % 2 == 0) {   // whole 32-column pieces: memory order
+            u = (w >> 3) * 4 + (w & 3);
+            half = (w >> 2) & 1;
+        } else {
+            u = w >> 1;
+            half = w & 1;
+        }
+        const int m = m0 + row, n = n0 + u * 8;
+        if (m < M && n < npad) *(f16x8 *)(O + m * ld + or_unit(n) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// The transpose: 16 columns (n0 ..) of the wave's 16 SM rows (m0 ..) become 16 rows of OT.
+template <int SM>
+__device__ __forceinline__ void or_store_cols(const f32x4 (&v)[SM], unsigned char *region, unsigned char *OT, long long ld, int m0, int n0, int M,
+                                              int N, int lane) {
+    constexpr int RS = SM * 64 + 16;
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < SM; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f16_t h, l;
+            or_split(m0 + i * 16 + r < M ? v[i][e] : 0.f, h, l);
+            unsigned char *p = region + (q * 4 + e) * RS + (i * 2 + (r >> 3)) * 32 + (r & 7) * 2;
+            *(f16_t *)p = h;
+            *(f16_t *)(p + 16) = l;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int mpad = or_chunks(M) * 32;
+#pragma unroll
+    for (int it0 = 0; it0 < 16 * SM * 4; it0 += 64) {
+        const int it = it0 + lane, row = it / (SM * 4), w = it - row * (SM * 4);
+        int u, half;
+        if (SM % 2 == 0) {
+            u = (w >> 3) * 4 + (w & 3);
+            half = (w >> 2) & 1;
+        } else {
+            u = w >> 1;
+            half = w & 1;
+        }
+        const int n = n0 + row, m = m0 + u * 8;
+        if (n < N && m < mpad) *(f16x8 *)(OT + n * ld + or_unit(m) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// WGM x WGN waves of 16 SM rows x 16 SN columns.  Two LDS slots of one 32-column stage each; per stage three products:
+//   hi hi (reading the lo fragments of R), hi lo (reading those of L), then the stage's one barrier - every wave holds all
+//   of the stage in registers, the next stage has landed - and lo hi, during which the next stage's hi fragments are read and
+//   the DMA of the stage after it runs into the slot just freed.
+template <int EPI, int WGM, int WGN, int SM, int SN>
+__global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
+    constexpr int W = WGM * WGN, T = WGM * SM * 16, OP = T * 128, PIECES = T / 8 / W;
+    static_assert(T == WGN * SN * 16 && PIECES * W * 8 == T, "square tiles, whole pieces per wave");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1, r = lane & 15, q = lane >> 4;
+    const int wm = wave / WGN, wn = wave % WGN, r = lane & 15, q = lane >> 4;
     constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
     const int per = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
     const int swz = xcd_remap(blockIdx.x, gridDim.x);
@@ -80,126 +164,169 @@ __global__ __launch_bounds__(256) void or_gemm_kernel(OrGemm g) {
         ti = t / g.tiles_n;
         tj = t - ti * g.tiles_n;
     }
+    ti = __builtin_amdgcn_readfirstlane(ti);
+    tj = __builtin_amdgcn_readfirstlane(tj);
     const int m0 = ti * T, n0 = tj * T;
     const long long ld = (long long)g.kc * 128;
-    const unsigned char *L = (z ? g.L[1] : g.L[0]) + b * g.sL, *R = g.R + b * g.sR;
 
-    auto fetch = [&](int s, unsigned char *slot) {
+    // DMA of a stage: the wave's pieces of 8 rows, wave + W p, rows behind the matrix clamped to its last one
+    const int prow = wave * 8 + (lane >> 3);
+    const unsigned chunk = (unsigned)(((lane & 7) ^ ((prow >> 1) & 7)) * 16), voff = (unsigned)(prow * ld) + chunk;
+    const unsigned step = (unsigned)(8 * W * ld);
+    const unsigned maxl = (unsigned)(min(g.M - 1 - m0, T - 1) * ld) + chunk, maxr = (unsigned)(min(g.N - 1 - n0, T - 1) * ld) + chunk;
+    const unsigned char *lbase = (z ? g.L[1] : g.L[0]) + b * g.sL + m0 * ld, *rbase = g.R + b * g.sR + n0 * ld;
+    const unsigned slots = (unsigned)(uintptr_t)LDS_PTR(lds) + wave * 1024;
+    auto fetch = [&](int s) {
+        const unsigned slot = slots + (s & 1) * (2 * OP);
 #pragma unroll
-        for (int p = wave; p < T / 8; p += 4) {
-            const int row = p * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-            const unsigned char *sl = L + min(m0 + row, g.M - 1) * ld + s * 128 + c * 16;
-            const unsigned char *sr = R + min(n0 + row, g.N - 1) * ld + s * 128 + c * 16;
-            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sl), LDS_PTR(slot + p * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(sr), LDS_PTR(slot + OP + p * 1024), 16, 0, 0);
+        for (int p = 0; p < PIECES; p++) {
+            p64_dma16(lbase, voff, p * step, maxl, slot + p * (W * 1024));
+            p64_dma16(rbase, voff, p * step, maxr, slot + OP + p * (W * 1024));
         }
+        lbase += 128;
+        rbase += 128;
     };
-    f32x4 acc[NT][NT];
+    f32x4 acc[SM][SN];
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+    for (int i = 0; i < SM; i++)
 #pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    fetch(0, lds);
+        for (int j = 0; j < SN; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    // lds_off of a row 16 further is 2048 bytes further, with the same chunk order
+    const int lh0 = lds_off(wm * SM * 16 + r, q), ll0 = lds_off(wm * SM * 16 + r, 4 + q);
+    const int rh0 = OP + lds_off(wn * SN * 16 + r, q), rl0 = OP + lds_off(wn * SN * 16 + r, 4 + q);
+    f16x8 lh[SM], ll[SM], rh[SN], rl[SN], rn[SN];
+    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (g.kc > 1) fetch(1);
+#pragma unroll
+    for (int i = 0; i < SM; i++) lh[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
+#pragma unroll
+    for (int j = 0; j < SN; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
     for (int s = 0; s < g.kc; s++) {
+        const unsigned char *cur = lds + (s & 1) * (2 * OP), *nxt = lds + ((s + 1) & 1) * (2 * OP);
+        // R first: a lane's four results are four consecutive columns of one row
+#pragma unroll
+        for (int j = 0; j < SN; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+#pragma unroll
+        for (int i = 0; i < SM; i++)
+#pragma unroll
+            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SM; i++) ll[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
+#pragma unroll
+        for (int i = 0; i < SM; i++)
+#pragma unroll
+            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < SM + SN; p++) {
+            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+        }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const unsigned char *cur = lds + (s & 1) * 2 * OP;
-        if (s + 1 < g.kc) fetch(s + 1, lds + ((s + 1) & 1) * 2 * OP);
-        f16x8 lh[NT], ll[NT], rh[NT], rl[NT];
+        if (s + 2 < g.kc) fetch(s + 2);
+        // behind the last stage these read what the slot held before: not used
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            lh[i] = *(const f16x8 *)(cur + lds_off(wm * WT + i * 16 + r, q));
-            ll[i] = *(const f16x8 *)(cur + lds_off(wm * WT + i * 16 + r, 4 + q));
-            rh[i] = *(const f16x8 *)(cur + OP + lds_off(wn * WT + i * 16 + r, q));
-            rl[i] = *(const f16x8 *)(cur + OP + lds_off(wn * WT + i * 16 + r, 4 + q));
+        for (int i = 0; i < SM; i++) lh[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
+#pragma unroll
+        for (int j = 0; j < SN; j++) rn[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
+#pragma unroll
+        for (int i = 0; i < SM; i++)
+#pragma unroll
+            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < SM + SN; p++) {
+            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
         }
-        // R first: a lane's four results are four consecutive columns of one row
 #pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
-            }
+        for (int j = 0; j < SN; j++) rh[j] = rn[j];
     }
 
     const float alpha = z ? g.alpha[1] : g.alpha[0];
-    unsigned char *O = (z ? g.O[1] : g.O[0]) + b * g.sO;
-    const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
+    const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16;
+    if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+        for (int i = 0; i < SM; i++)
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int m = m0 + wm * WT + i * 16 + r, n = n0 + wn * WT + j * 16 + q * 4;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] * alpha;
-            if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
+            for (int j = 0; j < SN; j++) {
+                const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
                 if (m >= g.M || n >= g.N) continue;
+                const f32x4 v = acc[i][j];
                 const long long at = m * g.ldo + n;
                 if constexpr (EPI == OR_OUT) {
                     bf16_t *o = (bf16_t *)g.out.p[b] + at;
                     if (g.wide) {
                         bf16x4 w;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) w[e] = (bf16_t)v[e];
+                        for (int e = 0; e < 4; e++) w[e] = (bf16_t)(v[e] * alpha);
                         *(bf16x4 *)o = w;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (n + e < g.N) o[e] = (bf16_t)v[e];
+                            if (n + e < g.N) o[e] = (bf16_t)(v[e] * alpha);
                     }
                 } else {
                     float *o = (float *)g.out.p[b] + at;
                     if (g.wide) {
                         float4 w = *(const float4 *)o;
-                        w.x = w.x * g.decay - g.rate * v[0];
-                        w.y = w.y * g.decay - g.rate * v[1];
-                        w.z = w.z * g.decay - g.rate * v[2];
-                        w.w = w.w * g.decay - g.rate * v[3];
+                        w.x = w.x * g.decay - g.rate * (v[0] * alpha);
+                        w.y = w.y * g.decay - g.rate * (v[1] * alpha);
+                        w.z = w.z * g.decay - g.rate * (v[2] * alpha);
+                        w.w = w.w * g.decay - g.rate * (v[3] * alpha);
                         *(float4 *)o = w;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (n + e < g.N) o[e] = o[e] * g.decay - g.rate * v[e];
+                            if (n + e < g.N) o[e] = o[e] * g.decay - g.rate * (v[e] * alpha);
                     }
                 }
-                continue;
             }
-            if constexpr (EPI == OR_POLY) {
-                if (m < g.M && n < or_chunks(g.N) * 32) {
-                    const unsigned char *a = g.A + b * g.sL + m * ld + (n >> 5) * 128 + (n & 31) * 2;
-                    const f16x4 ah = *(const f16x4 *)a, al = *(const f16x4 *)(a + 64);
+    } else {
+        unsigned char *O = (z ? g.O[1] : g.O[0]) + b * g.sO;
+        const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
+#pragma unroll
+        for (int i = 0; i < SM; i++)
+#pragma unroll
+            for (int j = 0; j < SN; j++) {
+                if constexpr (EPI == OR_POLY) {
+                    const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
+                    f16x4 ah = {0, 0, 0, 0}, al = ah;
+                    if (m < g.M && n < or_chunks(g.N) * 32) {
+                        const unsigned char *a = g.A + b * g.sL + m * ld + or_unit(n);
+                        ah = *(const f16x4 *)a;
+                        al = *(const f16x4 *)(a + 64);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        v[e] = g.cc * acc[i][j][e] + g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
+                        acc[i][j][e] = g.cc * acc[i][j][e] + g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] *= alpha;
                 }
             }
-            f16x4 hi, lo;
+        // the last stage's unused reads are done with the LDS (lgkmcnt), every wave has passed its last barrier's reads
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        unsigned char *region = lds + wave * (4 * OP / W);
+        static_assert(16 * (SM * 64 + 16) <= 4 * OP / W && 16 * (SN * 64 + 16) <= 4 * OP / W, "a wave's staging fits its share of the LDS");
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                f16_t h, l;
-                or_split(m < g.M && n + e < g.N ? v[e] : 0.f, h, l);
-                hi[e] = h;
-                lo[e] = l;
-            }
-            if (m < g.M && n < or_chunks(g.N) * 32) {
-                unsigned char *o = O + m * ldn + (n >> 5) * 128 + (n & 31) * 2;
-                *(f16x4 *)o = hi;
-                *(f16x4 *)(o + 64) = lo;
-            }
-            if ((EPI == OR_BOTH || ti != tj) && m < or_chunks(g.M) * 32) {
-                unsigned char *ot = (EPI == OR_BOTH ? g.OT + b * g.sOT : O) + (m >> 5) * 128 + (m & 31) * 2;
+        for (int i = 0; i < SM; i++) or_store_rows<SN>(acc[i], region, O, ldn, mw + i * 16, nw, g.M, g.N, lane);
+        if (EPI == OR_BOTH || ti != tj) {
+            unsigned char *OT = EPI == OR_BOTH ? g.OT + b * g.sOT : O;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (n + e < g.N) {
-                        *(f16_t *)(ot + (n + e) * ldm) = hi[e];
-                        *(f16_t *)(ot + (n + e) * ldm + 64) = lo[e];
-                    }
+            for (int j = 0; j < SN; j++) {
+                f32x4 col[SM];
+#pragma unroll
+                for (int i = 0; i < SM; i++) col[i] = acc[i][j];
+                or_store_cols<SM>(col, region, OT, ldm, mw, nw + j * 16, g.M, g.N, lane);
             }
         }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -415,6 +542,14 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
     return or_exponent(top, o.ex[o.blocks]);
 }
 
+template <int EPI, int WGM, int WGN, int SM, int SN>
+static int or_launch_tile(const OrGemm &g, long long blocks, int products, hipStream_t stream) {
+    constexpr int LDS = 4 * WGM * SM * 16 * 128;
+    if (!lds_attr((const void *)or_gemm_kernel<EPI, WGM, WGN, SM, SN>, LDS)) return SGCLIP_ELAUNCH;
+    or_gemm_kernel<EPI, WGM, WGN, SM, SN><<<dim3((unsigned)blocks, 1, products), 64 * WGM * WGN, LDS, stream>>>(g);
+    return launch_check("sgclip_orthogonalize");
+}
+
 template <int EPI>
 static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t stream) {
     OrGemm g = gin;
@@ -424,20 +559,17 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
         g.tiles_n = ceil_div(g.N, T);
         return (long long)batch * (SYM ? (long long)g.tiles_m * (g.tiles_m + 1) / 2 : (long long)g.tiles_m * g.tiles_n);
     };
-    // 128 x 128 tiles where they fill the chip, 64 x 64 below that
-    long long blocks = tiles(128);
-    if (blocks * products * 4 * 256 > 0xffffffffLL) {   // 64 x 64 tiles at most; a launch counts its threads in 32 bits
+    if (tiles(64) * products * 256 > 0xffffffffLL) {   // a launch counts its threads in 32 bits
         set_error("sgclip_orthogonalize: %d matrices of %d x %d are more than one launch holds", batch, g.M, g.N);
         return SGCLIP_EINVAL;
     }
-    if (blocks * products >= device_cus()) {
-        if (!lds_attr((const void *)or_gemm_kernel<EPI, 64>, 4 * 128 * 128)) return SGCLIP_ELAUNCH;
-        or_gemm_kernel<EPI, 64><<<dim3((unsigned)blocks, 1, products), 256, 4 * 128 * 128, stream>>>(g);
-    } else {
-        blocks = tiles(64);
-        or_gemm_kernel<EPI, 32><<<dim3((unsigned)blocks, 1, products), 256, 4 * 64 * 128, stream>>>(g);
-    }
-    return launch_check("sgclip_orthogonalize");
+    const int cus = device_cus();
+    static const int force = getenv("OR_TILE") ? atoi(getenv("OR_TILE")) : 0;
+    if (force == 256) return or_launch_tile<EPI, 2, 4, 8, 4>(g, tiles(256), products, stream);
+    if (force == 192) return or_launch_tile<EPI, 2, 4, 6, 3>(g, tiles(192), products, stream);
+    if (force == 128) return or_launch_tile<EPI, 2, 2, 4, 4>(g, tiles(128), products, stream);
+    if (tiles(128) * products >= cus) return or_launch_tile<EPI, 2, 2, 4, 4>(g, tiles(128), products, stream);
+    return or_launch_tile<EPI, 2, 2, 2, 2>(g, tiles(64), products, stream);
 }
 
 static inline float or_pow2(int e) { return ldexpf(1.0f, e); }

@@ -111,6 +111,28 @@ def test_linear_against_64_bits(M, N, K, dtype):
            size + b.double().abs() + r.double().abs(), K, 2)
 
 
+@pytest.mark.parametrize("M,N,K", [(4200, 4100, 200), (4097, 4096, 512), (8192, 2560, 700), (16500, 1028, 1300), (33000, 512, 64)])
+def test_linear_many_tiles(M, N, K):
+    """More 256 x 256 tiles than compute units: several tiles per workgroup, ragged in both directions, one to six stages each."""
+    x, w = _x(M, K, BF16), 0.02 * torch.randn(N, K, device="cuda")
+    b, r = torch.randn(N, device="cuda"), torch.randn(M, N, device="cuda")
+    xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    xv, wv = values(x), values(w)
+    s, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    y = ops.linear_mxfp4(xq, wq, b, residual=r)
+    _check(y, r.double() + s + b.double(), size + b.double().abs() + r.double().abs(), K, 2)
+    again = r.clone()
+    assert torch.equal(ops.linear_mxfp4(x, wq, b, residual=again, out=again), y)
+    _check(ops.linear_mxfp4(xq, wq), s, size, K, 0, UBF * (s.abs() + K * U32 * size))
+    u = s + b.double()
+    g = u * torch.sigmoid(1.702 * u)
+    err = 1.1 * (K + 1) * U32 * (size + b.double().abs()) + 2.0 ** -20 * g.abs()
+    y = ops.linear_mxfp4(xq, wq, b, gelu=True)
+    _check(y, g, 0 * size, 0, 0, err + UBF * (g.abs() + err))
+    for _ in range(3):
+        assert torch.equal(ops.linear_mxfp4(xq, wq, b, gelu=True), y)
+
+
 def test_linear_views_in_place_and_untouched_neighbours():
     M, N, K = 70, 96, 160
     x = _x(2 * M, K + 9, BF16)[::2, 5:5 + K]
