@@ -10,6 +10,7 @@
 // the scales of 64 rows x 4 blocks as one contiguous 256-byte load, and the instruction picks the byte of its 16 rows itself.
 #include "tile_common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace sgclip {
@@ -48,34 +49,41 @@ __device__ __forceinline__ unsigned mx_codes8(const float (&v)[8], unsigned byte
     return r;
 }
 
-// Eight elements from column k of a row (zeros behind cols).  VEC: 16-byte loads, whole groups of eight only.
-template <typename T, bool VEC>
-__device__ __forceinline__ void mx_load8(const T *__restrict__ row, int k, int cols, float (&v)[8]) {
+// Eight elements of a row as they lie in memory.
+template <typename T>
+struct MxRaw {
+    T v[8] __attribute__((aligned(16)));
+};
+
+// Eight elements from column k of a row (zeros behind cols).  VEC: 16-byte loads, whole groups of eight only.  STREAM: the
+// elements are not needed again (non-temporal).
+template <typename T, bool VEC, bool STREAM = false>
+__device__ __forceinline__ MxRaw<T> mx_load8(const T *__restrict__ row, int k, int cols) {
+    MxRaw<T> x;
     if constexpr (VEC) {
-        if (k < cols) {
-            if constexpr (std::is_same<T, float>::value) {
-                const float4 a = *(const float4 *)(row + k), b = *(const float4 *)(row + k + 4);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-            } else {
-                const bf16x8 a = *(const bf16x8 *)(row + k);
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = (float)a[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.f;
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) {
+            const u32x4 *p = (const u32x4 *)(row + k) + j;
+            ((u32x4 *)x.v)[j] = k < cols ? (STREAM ? __builtin_nontemporal_load(p) : *p) : (u32x4){0, 0, 0, 0};
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = k + j < cols ? (float)row[k + j] : 0.f;
+        for (int j = 0; j < 8; j++) x.v[j] = k + j < cols ? row[k + j] : (T)0.f;
     }
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void mx_floats(const MxRaw<T> &x, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = (float)x.v[j];
 }
 
 // ---------------------------------------------------------------------------
 // Quantisation: a workgroup takes 64 rows x 256 columns, so that the tile's scales are 512 contiguous bytes; four lanes share
 // a block of 32 and find its maximum with two exchanges.  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written
-// per element.
+// per element; 73856 x 1024 bf16 in 32 us (6.0 TB/s; 46 us with ordinary loads converted at once).
 // ---------------------------------------------------------------------------
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, long long ldx, int rows, int cols,
@@ -86,11 +94,11 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ 
     const int kt = (int)(kp / MX_K);
     const int rb = blockIdx.x / kt, kb = blockIdx.x % kt;
     const int c = tid & 31, k = kb * MX_K + c * 8;
-    float v[8][8];
+    MxRaw<T> raw[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int row = rb * 64 + (tid >> 5) + 8 * i;
-        if (row < rows) mx_load8<T, VEC>(x + row * ldx, k, cols, v[i]);
+        raw[i] = mx_load8<T, VEC, true>(x + min(row, rows - 1) * ldx, k, cols);
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -99,13 +107,15 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ 
             if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = 0;
             continue;
         }
+        float v[8];
+        mx_floats(raw[i], v);
         unsigned am = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[j]) & 0x7fffffffu);
         am = max(am, (unsigned)__shfl_xor((int)am, 1, 64));
         am = max(am, (unsigned)__shfl_xor((int)am, 2, 64));
         const unsigned byte = mx_scale_byte(am);
-        *(unsigned *)(codes + row * (kp / 2) + (k >> 1)) = mx_codes8(v[i], byte);
+        *(unsigned *)(codes + row * (kp / 2) + (k >> 1)) = mx_codes8(v, byte);
         if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = (unsigned char)byte;
     }
     __syncthreads();
@@ -191,7 +201,9 @@ struct MxGemm {
     int wide;    // out, bias, resid allow four columns per access
 };
 
-__device__ __forceinline__ float mx_gelu(float x) { return x / (1.0f + __expf(-1.702f * x)); }
+// x sigmoid(1.702 x) on the hardware's exp2 and reciprocal (a few 2^-24, far below the bf16 rounding that follows; with an exact
+// division the large product spends 150 us more in its epilogue)
+__device__ __forceinline__ float mx_gelu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.4554669595930156f * x)); }
 
 enum { MX_BF16 = 0, MX_GELU = 1, MX_RESID = 2 };
 
@@ -309,12 +321,10 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
 // Many tiles: persistent workgroups, 256 x 256 tiles, eight waves of 128 rows x 64 columns.
 // The stages of a workgroup's tiles form one stream through two LDS slots; a stage is two 128-deep sub-steps whose fragments are
 // double-buffered in registers, with one barrier between them: there every wave holds all of stage g, stage g + 1 has landed,
-// and the DMA of stage g + 2 (of the next tile, if need be) starts into the slot just freed.  A tile's results leave through
-// a staging area of their own, so the next tile's operands arrive meanwhile; the barrier after them waits for the
-// fetches only (they are older than the stores, and the counter retires in order).
+// and the DMA of stage g + 2 (of the next tile, if need be) starts into the slot just freed.  A tile's results leave from the registers
+// while the next tile's operands arrive; the barrier after them waits for the fetches only (they are older than the stores, and the counter retires in order).
 // ---------------------------------------------------------------------------
-constexpr int MXP_OP = 256 * 128, MXP_SLOT = 2 * MXP_OP + 4096, MXP_BIAS = 2 * MXP_SLOT, MXP_STAGE = MXP_BIAS + 4096, MXP_ROW = 144;
-constexpr int MXP_LDS = MXP_STAGE + 8 * 16 * MXP_ROW;
+constexpr int MXP_OP = 256 * 128, MXP_SLOT = 2 * MXP_OP + 4096, MXP_BIAS = 2 * MXP_SLOT, MXP_LDS = MXP_BIAS + 4096;
 static_assert(MXP_LDS <= 160 * 1024, "LDS of a CU");
 
 struct MxFrags {
@@ -354,56 +364,47 @@ constexpr int mxp_stores() {
     return EPI == MX_RESID ? 32 : 16;
 }
 
+// Straight from the registers: for bf16 two neighbouring 16-lane rows exchange halves, after which a lane holds eight consecutive
+// columns (64 bytes of a row per instruction; through LDS the 16 round trips of a tile cost 2 us).  Non-temporal: ordinary
+// stores wait for the evictions of the previous tile's lines (73856 x 1024 x 4096: 267 us, non-temporal 223).
 template <int EPI>
-__device__ __forceinline__ void mxp_epilogue(const MxGemm &g, f32x4 (&acc)[8][4], const unsigned char *bias, unsigned char *region, int mw, int nw,
-                                             int lane) {
+__device__ __forceinline__ void mxp_epilogue(const MxGemm &g, const f32x4 (&acc)[8][4], const unsigned char *bias, int mw, int nw, int lane) {
     const int r = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if constexpr (EPI == MX_RESID) {
+    for (int p = 0; p < 2; p++) {
+        f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
+        if (g.bias) {
+            b0 = *(const f32x4 *)(bias + (p * 32 + q * 4) * 4);
+            b1 = *(const f32x4 *)(bias + (p * 32 + 16 + q * 4) * 4);
+        }
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
+        for (int i = 0; i < 8; i++) {
+            const int m = mw + i * 16 + r;
+            const f32x4 v0 = acc[i][2 * p] + b0, v1 = acc[i][2 * p + 1] + b1;
+            if constexpr (EPI == MX_RESID) {
+                const int n = nw + p * 32 + q * 4;
+                if (m < g.M && n < g.N)
+                    __builtin_nontemporal_store(*(const f32x4 *)(g.resid + m * g.ldr + n) + v0, (f32x4 *)((float *)g.out + m * g.ldo + n));
+                if (m < g.M && n + 16 < g.N)
+                    __builtin_nontemporal_store(*(const f32x4 *)(g.resid + m * g.ldr + n + 16) + v1, (f32x4 *)((float *)g.out + m * g.ldo + n + 16));
+            } else {
+                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+                bf16x4 o0, o1;
 #pragma unroll
-                for (int jj = 0; jj < 2; jj++) {
-                    const int j = half * 2 + jj;
-                    f32x4 v = acc[i][j];
-                    if (g.bias) v += *(const f32x4 *)(bias + (j * 16 + q * 4) * 4);
-                    *(f32x4 *)(region + r * MXP_ROW + jj * 64 + q * 16) = v;
+                for (int e = 0; e < 4; e++) {
+                    o0[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v0[e]) : v0[e]);
+                    o1[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v1[e]) : v1[e]);
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int row = (lane >> 3) + 8 * h, m = mw + i * 16 + row, n = nw + half * 32 + (lane & 7) * 4;
-                    const f32x4 v = *(const f32x4 *)(region + row * MXP_ROW + (lane & 7) * 16);
-                    if (m < g.M && n < g.N) {
-                        const f32x4 rv = *(const f32x4 *)(g.resid + m * g.ldr + n);
-                        *(f32x4 *)((float *)g.out + m * g.ldo + n) = rv + v;
-                    }
-                }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                f32x4 v = acc[i][j];
-                if (g.bias) v += *(const f32x4 *)(bias + (j * 16 + q * 4) * 4);
-                bf16x4 o;
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v[e]) : v[e]);
-                *(bf16x4 *)(region + r * MXP_ROW + j * 32 + q * 8) = o;
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int row = (lane >> 3) + 8 * h, m = mw + i * 16 + row, n = nw + (lane & 7) * 8;
-                const bf16x8 v = *(const bf16x8 *)(region + row * MXP_ROW + (lane & 7) * 16);
+                const u32x2 w0 = __builtin_bit_cast(u32x2, o0), w1 = __builtin_bit_cast(u32x2, o1);
+                const u32x2 lo = __builtin_amdgcn_permlane16_swap(w0[0], w1[0], false, false), hi = __builtin_amdgcn_permlane16_swap(w0[1], w1[1], false, false);
+                const int n = nw + p * 32 + (q & 1) * 16 + (q >> 1) * 8;
                 if (m < g.M && n < g.N) {
                     bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
-                    if (n + 8 <= g.N) *(bf16x8 *)o = v;
-                    else *(bf16x4 *)o = (bf16x4){v[0], v[1], v[2], v[3]};
+                    if (n + 8 <= g.N) __builtin_nontemporal_store((u32x4){lo[0], hi[0], lo[1], hi[1]}, (u32x4 *)o);
+                    else *(u32x2 *)o = (u32x2){lo[0], hi[0]};
                 }
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     }
 }
@@ -499,27 +500,27 @@ __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, i
         }
         int m0, n0;
         origin(t, m0, n0);
-        mxp_epilogue<EPI>(g, acc, lds + MXP_BIAS + bias * 1024 + wn * 256, lds + MXP_STAGE + wave * (16 * MXP_ROW), m0 + wm * 128, n0 + wn * 64, lane);
+        mxp_epilogue<EPI>(g, acc, lds + MXP_BIAS + bias * 1024 + wn * 256, m0 + wm * 128, n0 + wn * 64, lane);
         bias = (bias + 1) & 3;
         stored = m0 + 256 <= g.M && n0 + 256 <= g.N;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// Up to 16 rows of x, quantised on the way in: a workgroup takes 16 columns of y, its eight waves 128-deep slices of K in turn,
-// and joins their sums through LDS.  A lane holds one block of 32 of one row, so the block's maximum needs no exchange.
+// Up to 16 rows of x, quantised on the way in: a workgroup takes 16 columns of y, its waves (one per 128 of K, at most 16)
+// 128-deep slices of K in turn, and joins their sums through LDS.  A lane holds one block of 32 of one row, so the block's maximum needs no exchange.
 // Bound by the weights' bytes (and, below about a megabyte of them, by the launch).
 template <typename T, bool VEC, int EPI>
-__global__ __launch_bounds__(512) void mx_few_rows_kernel(const T *__restrict__ x, long long ldx, int K, MxGemm g) {
-    __shared__ f32x4 part[8][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+__global__ __launch_bounds__(1024) void mx_few_rows_kernel(const T *__restrict__ x, long long ldx, int K, MxGemm g) {
+    __shared__ f32x4 part[16][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16;
     const long long ld = g.kp / 2;
     const int nrow = min(n0 + r, g.N - 1);
     const unsigned char *wc = g.wc + nrow * ld;
     f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
     const int steps = (K + 127) / 128;
-    for (int s = wave; s < steps; s += 8) {
+    for (int s = wave; s < steps; s += waves) {
         const int block = s * 4 + q;
         const i32x4 fw = *(const i32x4 *)(wc + block * 16);
         const unsigned sw = g.ws[(((long long)(nrow >> 6) * (g.kp / 32) + block) * 16 + (nrow & 15)) * 4 + ((nrow & 63) >> 4)];
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(const T *__restrict__ 
             unsigned am = 0;
 #pragma unroll
             for (int p = 0; p < 4; p++) {
-                mx_load8<T, VEC>(x + r * ldx, block * 32 + p * 8, K, v[p]);
+                mx_floats(mx_load8<T, VEC>(x + r * ldx, block * 32 + p * 8, K), v[p]);
 #pragma unroll
                 for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[p][j]) & 0x7fffffffu);
             }
@@ -543,8 +544,7 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(const T *__restrict__ 
     part[wave][lane] = acc;
     __syncthreads();
     if (wave == 0) {
-#pragma unroll
-        for (int w = 1; w < 8; w++) acc += part[w][lane];
+        for (int w = 1; w < waves; w++) acc += part[w][lane];
         mx_store4<EPI>(g, acc, r, n0 + q * 4);
     }
 }
@@ -611,9 +611,9 @@ static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
 template <typename T, int EPI>
 static void mx_launch_few(const T *x, long long ldx, int K, const MxGemm &g, hipStream_t stream) {
     const bool vec = K % 8 == 0 && ldx * sizeof(T) % 16 == 0 && ((uintptr_t)x & 15) == 0;
-    const dim3 grid((unsigned)((g.N + 15) / 16));
-    if (vec) mx_few_rows_kernel<T, true, EPI><<<grid, 512, 0, stream>>>(x, ldx, K, g);
-    else mx_few_rows_kernel<T, false, EPI><<<grid, 512, 0, stream>>>(x, ldx, K, g);
+    const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * std::min(16, (K + 127) / 128));
+    if (vec) mx_few_rows_kernel<T, true, EPI><<<grid, block, 0, stream>>>(x, ldx, K, g);
+    else mx_few_rows_kernel<T, false, EPI><<<grid, block, 0, stream>>>(x, ldx, K, g);
 }
 
 static int mx_epilogue(const char *who, MxGemm &g, int epilogue, const float *bias, const float *aux, int64_t ldaux, void *out, int64_t ldo,
