@@ -401,6 +401,12 @@ int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void 
                         int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
                         void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* out[n] = sum_m in[m][n] (in bf16 or f32 [M, N], row stride ld; out f32) in an order that does not change between calls: the
+ * bias gradient of the layer. */
+size_t sgclip_column_sums_workspace_bytes(int M, int N);
+int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int N, float *out_dev, void *workspace_dev,
+                       size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------------
  * (8) Orthogonalised updates (the Muon optimiser's step).  No counterpart in the reference, which trains with Adam
  * (scripts/train_sgclip.py:232-241); for the weight matrices of the same linear layers.

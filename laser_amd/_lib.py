@@ -127,6 +127,8 @@ SIGNATURES = {
     "sgclip_mxfp4_linear_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "sgclip_mxfp4_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                       C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "sgclip_column_sums_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "sgclip_column_sums": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "sgclip_orthogonalize_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "sgclip_orthogonalize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
                                        C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),

@@ -550,6 +550,46 @@ __global__ __launch_bounds__(1024) void mx_few_rows_kernel(const T *__restrict__
 }
 
 // ---------------------------------------------------------------------------
+// Column sums without atomics (bias gradients): every workgroup sums a strip of rows of 512 columns (a lane eight of them, its
+// four waves every fourth row), a second launch adds the strips in order.  Bound by HBM: 36928 x 4096 bf16.
+// ---------------------------------------------------------------------------
+constexpr int CS_COLS = 512, CS_STRIPS = 256, CS_ROWS = 32;
+
+static inline int cs_strips(int M) { return std::max(1, std::min(CS_STRIPS, (M + CS_ROWS - 1) / CS_ROWS)); }
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void mx_colsum_strip_kernel(const T *__restrict__ in, long long ld, int M, int N, float *__restrict__ parts) {
+    __shared__ float sums[4][CS_COLS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * CS_COLS + lane * 8;
+    const long long per = ((long long)M + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per, hi = min(lo + per, (long long)M);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < N) {
+#pragma unroll 4
+        for (long long m = lo + wave; m < hi; m += 4) {
+            float v[8];
+            mx_floats(mx_load8<T, VEC>(in + m * ld, n, N), v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) s[j] += v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) sums[wave][lane * 8 + j] = s[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < CS_COLS; c += 256)
+        if (blockIdx.x * CS_COLS + c < N)
+            parts[(long long)blockIdx.y * N + blockIdx.x * CS_COLS + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+}
+
+__global__ __launch_bounds__(64) void mx_colsum_join_kernel(const float *__restrict__ parts, int strips, int N, float *__restrict__ out) {
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (n >= N) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < strips; i++) s += parts[(long long)i * N + n];
+    out[n] = s;
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 static bool mx_shape_ok(const char *who, int rows, int cols) {
@@ -751,6 +791,41 @@ int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void 
     else if (epi == MX_GELU) f32 ? mx_launch_few<float, MX_GELU>(xf, ldx, K, g, st) : mx_launch_few<bf16_t, MX_GELU>(xb, ldx, K, g, st);
     else f32 ? mx_launch_few<float, MX_RESID>(xf, ldx, K, g, st) : mx_launch_few<bf16_t, MX_RESID>(xb, ldx, K, g, st);
     return launch_check("sgclip_mxfp4_linear");
+}
+
+size_t sgclip_column_sums_workspace_bytes(int M, int N) {
+    return M <= 0 || N <= 0 ? 0 : (size_t)cs_strips(M) * (size_t)N * sizeof(float);
+}
+
+int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int N, float *out_dev, void *workspace_dev, size_t workspace_bytes,
+                       void *stream) {
+    if (N == 0) return SGCLIP_OK;
+    if (M < 0 || N < 0 || (M > 0 && !in_dev) || !out_dev || ld < N || (in_dtype != SGCLIP_DTYPE_F32 && in_dtype != SGCLIP_DTYPE_BF16)) {
+        set_error("sgclip_column_sums: bad arguments M=%d N=%d ld=%lld dtype=%d", M, N, (long long)ld, in_dtype);
+        return SGCLIP_EINVAL;
+    }
+    if (M > 0 && (!workspace_dev || workspace_bytes < sgclip_column_sums_workspace_bytes(M, N))) {
+        set_error("sgclip_column_sums: workspace of %zu bytes, %zu needed", workspace_dev ? workspace_bytes : (size_t)0,
+                  sgclip_column_sums_workspace_bytes(M, N));
+        return SGCLIP_ENOSPC;
+    }
+    const int strips = M > 0 ? cs_strips(M) : 0;
+    hipStream_t st = (hipStream_t)stream;
+    float *parts = (float *)workspace_dev;
+    const dim3 grid((unsigned)ceil_div(N, CS_COLS), (unsigned)strips);
+    if (strips) {
+        const size_t size = in_dtype == SGCLIP_DTYPE_F32 ? 4 : 2;
+        const bool vec = N % 8 == 0 && ld * size % 16 == 0 && ((uintptr_t)in_dev & 15) == 0;
+        if (in_dtype == SGCLIP_DTYPE_F32) {
+            if (vec) mx_colsum_strip_kernel<float, true><<<grid, 256, 0, st>>>((const float *)in_dev, ld, M, N, parts);
+            else mx_colsum_strip_kernel<float, false><<<grid, 256, 0, st>>>((const float *)in_dev, ld, M, N, parts);
+        } else {
+            if (vec) mx_colsum_strip_kernel<bf16_t, true><<<grid, 256, 0, st>>>((const bf16_t *)in_dev, ld, M, N, parts);
+            else mx_colsum_strip_kernel<bf16_t, false><<<grid, 256, 0, st>>>((const bf16_t *)in_dev, ld, M, N, parts);
+        }
+    }
+    mx_colsum_join_kernel<<<dim3((unsigned)((N + 63) / 64)), 64, 0, st>>>(parts, strips, N, out_dev);
+    return launch_check("sgclip_column_sums");
 }
 
 }  // extern "C"

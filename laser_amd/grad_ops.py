@@ -252,6 +252,20 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: Optional[torch.Tensor] 
 
 
 # -- linear layers in 4-bit floats -----------------------------------------------------------
+def column_sums(x: torch.Tensor) -> torch.Tensor:
+    """f32 [N] column sums of x [M, N] (bf16 or f32), the same bits at every call (`colsum` adds with atomics, and to its output)."""
+    if x.dim() != 2 or not x.is_cuda or (x.numel() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]))):
+        raise ValueError(f"column_sums: expected [M, N] with contiguous rows on the GPU, got {tuple(x.shape)} {x.stride()} on {x.device}")
+    M, N = x.shape
+    lib = _lib.load()
+    need = lib.sgclip_column_sums_workspace_bytes(M, N)
+    out = torch.empty(N, dtype=F32, device=x.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.check(lib.sgclip_column_sums(x.data_ptr(), _dtype_code(x), x.stride(0) if M > 1 else max(N, 1), M, N, out.data_ptr(), _ptr(ws), need,
+                                      _stream(x)))
+    return out
+
+
 def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dtype = BF16, need_dx: bool = True, need_dw: bool = True,
                      need_db: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw, db) of y = xq wq^T + b for dy bf16 / f32 [M, N]: the gradient in the quantised operands, which a straight-through
@@ -261,20 +275,15 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
         raise ValueError(f"linear_mxfp4_bwd: dy {dy.dtype} {tuple(dy.shape)} for x {xq.shape} and weight {wq.shape}")
     if dx_dtype not in (BF16, F32):
         raise ValueError(f"linear_mxfp4_bwd: dx in {dx_dtype}")
-    _same_device(dy, xq.codes, wq.codes)
+    _same_device(dy, xq.data, wq.data)
     dy = dy.contiguous()
     M, N, K = xq.rows, wq.rows, xq.cols
     dev = dy.device
-    db = torch.zeros(N, dtype=F32, device=dev) if need_db else None
+    db = column_sums(dy) if need_db else None
     if M == 0:
         return (torch.empty((0, K), dtype=dx_dtype, device=dev) if need_dx else None,
                 torch.zeros((N, K), dtype=F32, device=dev) if need_dw else None, db)
-    if dy.dtype == F32:
-        dyb = cast_bf16_colsum(dy, db) if need_db else cast_bf16(dy)
-    else:
-        dyb = dy
-        if need_db:
-            colsum(dy, db)
+    dyb = cast_bf16(dy) if dy.dtype == F32 else dy
     dx = None
     if need_dx:
         w_t = dequantize_mxfp4(wq, transpose=True)       # [K, N rounded up to 64], zeros behind N

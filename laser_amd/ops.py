@@ -21,10 +21,15 @@ def _stream(t: Optional[torch.Tensor] = None) -> int:
     kernel will touch: its device must be the current one (HIP launches on the current device; a pointer of
     another GPU would fault there), so callers with tensors elsewhere run under `torch.cuda.device(...)`,
     as PredicateModel does for its own device."""
-    if t is not None and t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensor on {t.device} but the current HIP device is cuda:{torch.cuda.current_device()}: "
+    device = torch.cuda.current_device()
+    if t is not None and t.device.index != device:
+        raise RuntimeError(f"tensor on {t.device} but the current HIP device is cuda:{device}: "
                            f"run this call under torch.cuda.device({t.device.index})")
-    return torch.cuda.current_stream().cuda_stream
+    # the handle itself where torch hands it out: a Stream object costs 2 us, as much as a launch
+    return _RAW_STREAM(device) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
+
+
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -328,20 +333,22 @@ def topk_columns(probs: torch.Tensor, k: int, tie_rank: Optional[torch.Tensor] =
 # ---------------------------------------------------------------------------
 # microscaled 4-bit linear layers
 # ---------------------------------------------------------------------------
-def _rows2d(name: str, t: torch.Tensor, dtypes) -> torch.Tensor:
-    """t, checked to be a 2-D device tensor of one of `dtypes` whose rows are contiguous and do not overlap."""
+_MX_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _rows2d(name: str, t: torch.Tensor, dtypes) -> int:
+    """Row stride of t, checked to be a 2-D device tensor of one of `dtypes` whose rows are contiguous and do not overlap (a
+    single row may carry any stride)."""
     if t.dim() != 2 or t.dtype not in dtypes:
         raise ValueError(f"{name}: expected a 2-D tensor of {' or '.join(str(d) for d in dtypes)}, got {t.dtype} {tuple(t.shape)}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: expected a tensor on the GPU, got {t.device}")
-    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if rows <= 1:
+        ld = cols
+    if (cols > 1 and rows and step != 1) or ld < cols:
         raise ValueError(f"{name}: rows must be contiguous and apart, got strides {t.stride()} for {tuple(t.shape)}")
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride of a checked 2-D tensor (a single row may carry any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    return ld if ld > 0 else 1
 
 
 def _same_device(a: torch.Tensor, *others: Optional[torch.Tensor]):
@@ -367,16 +374,36 @@ def _apart(name: str, out: torch.Tensor, *inputs: Optional[torch.Tensor]):
 
 class Mxfp4:
     """A [rows, cols] matrix in microscaled 4-bit floats: 4-bit elements (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives) with
-    one power-of-two scale per 32 consecutive elements of a row; 17/32 byte an element.  `codes` and `scales` (u8, on the
-    GPU) are in the order include/sgclip.h describes; make one with `quantize_mxfp4`, read it with `dequantize_mxfp4`."""
+    one power-of-two scale per 32 consecutive elements of a row; 17/32 byte an element.  `data` (u8, on the GPU) holds the
+    codes and behind them the scales, in the order include/sgclip.h describes; make one with `quantize_mxfp4`, read it with
+    `dequantize_mxfp4`."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
-        lib = _lib.load()
-        for t, need in ((codes, lib.sgclip_mxfp4_codes_bytes(rows, cols)), (scales, lib.sgclip_mxfp4_scales_bytes(rows, cols))):
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != need or t.device.type != "cuda":
-                raise ValueError(f"4-bit [{rows}, {cols}]: expected {need} contiguous bytes on the GPU, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        _same_device(codes, scales)
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+    __slots__ = ("data", "rows", "cols", "split")
+
+    def __init__(self, data: torch.Tensor, rows: int, cols: int):
+        codes, scales = self.sizes(rows, cols)
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != codes + scales or not data.is_cuda or data.data_ptr() % 16:
+            raise ValueError(f"4-bit [{rows}, {cols}]: expected {codes + scales} contiguous bytes on the GPU, got {data.dtype} "
+                             f"{tuple(data.shape)} on {data.device}")
+        self.data, self.rows, self.cols, self.split = data, rows, cols, codes
+
+    @staticmethod
+    def sizes(rows: int, cols: int):
+        """Bytes of the codes and of the scales (sgclip_mxfp4_codes_bytes, sgclip_mxfp4_scales_bytes)."""
+        kp = (cols + 255) // 256 * 256
+        return rows * (kp // 2), (rows + 63) // 64 * 64 * (kp // 32)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[: self.split]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.split:]
+
+    def pointers(self):
+        p = self.data.data_ptr()
+        return p, p + self.split
 
     @property
     def shape(self):
@@ -384,37 +411,36 @@ class Mxfp4:
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
 
 
 def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     """x [rows, cols] (bf16 or f32, contiguous rows of any stride) in 4-bit floats.  A block's scale is
     2^(floor(log2 max|x|) - 2); elements round to the nearest value, ties to the even code, above 6 scales to 6.  A block
     of 32 that holds an infinity or a NaN reads back as NaN."""
-    lib = _lib.load()
-    _rows2d("quantize_mxfp4", x, (torch.bfloat16, torch.float32))
+    ld = _rows2d("quantize_mxfp4", x, _MX_DTYPES)
     rows, cols = x.shape
     if cols == 0:
         raise ValueError("quantize_mxfp4: rows of no elements")
-    codes = torch.empty(lib.sgclip_mxfp4_codes_bytes(rows, cols), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(lib.sgclip_mxfp4_scales_bytes(rows, cols), dtype=torch.uint8, device=x.device)
-    _lib.check(lib.sgclip_mxfp4_quantize(x.data_ptr(), _lib.DTYPE_F32 if x.dtype == torch.float32 else _lib.DTYPE_BF16, _ld(x), rows, cols,
-                                         codes.data_ptr(), scales.data_ptr(), _stream(x)))
-    return Mxfp4(codes, scales, rows, cols)
+    codes, scales = Mxfp4.sizes(rows, cols)
+    q = Mxfp4(torch.empty(codes + scales, dtype=torch.uint8, device=x.device), rows, cols)
+    p, s = q.pointers()
+    _lib.check(_lib.load().sgclip_mxfp4_quantize(x.data_ptr(), _MX_DTYPES[x.dtype], ld, rows, cols, p, s, _stream(x)))
+    return q
 
 
 def dequantize_mxfp4(q: Mxfp4, transpose: bool = False) -> torch.Tensor:
     """The values of q in bf16 (exact): [rows, cols], or with transpose [cols, ld] with out[k, r] = q[r, k] and zeros in the
     columns from rows to ld = rows rounded up to 64 (the reduction padding `gemm_bf16` asks for)."""
-    lib = _lib.load()
-    shape = (q.cols, (q.rows + 63) // 64 * 64) if transpose else (q.rows, q.cols)
-    out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-    _lib.check(lib.sgclip_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, 1 if transpose else 0, out.data_ptr(),
-                                           shape[1], _stream(q.codes)))
+    rows, cols = q.rows, q.cols
+    ld = (rows + 63) // 64 * 64 if transpose else cols
+    out = torch.empty((cols if transpose else rows, ld), dtype=torch.bfloat16, device=q.device)
+    p, s = q.pointers()
+    _lib.check(_lib.load().sgclip_mxfp4_dequantize(p, s, rows, cols, 1 if transpose else 0, out.data_ptr(), ld, _stream(q.data)))
     return out
 
 
@@ -425,41 +451,38 @@ def linear_mxfp4(x, w: Mxfp4, bias: Optional[torch.Tensor] = None, *, gelu: bool
     sum residual + x w^T + bias, which may go into the residual itself (out=residual).  One launch up to 16 rows of x."""
     lib = _lib.load()
     quantised = isinstance(x, Mxfp4)
-    if not quantised:
-        _rows2d("linear_mxfp4: x", x, (torch.bfloat16, torch.float32))
+    xt = x.data if quantised else x
+    ldx = 0 if quantised else _rows2d("linear_mxfp4: x", x, _MX_DTYPES)
     M, K = x.shape
     N = w.rows
     if K != w.cols:
         raise ValueError(f"linear_mxfp4: x has {K} columns, the weight {w.cols}")
-    if gelu and residual is not None:
-        raise ValueError("linear_mxfp4: gelu and residual exclude each other")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
+    dtype, epi, ldr = torch.bfloat16, _lib.EPI_BIAS_GELU_BF16 if gelu else _lib.EPI_BIAS_BF16, 0
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
         raise ValueError(f"linear_mxfp4: bias must be contiguous f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
-    dtype = torch.float32 if residual is not None else torch.bfloat16
     if residual is not None:
-        _rows2d("linear_mxfp4: residual", residual, (torch.float32,))
+        if gelu:
+            raise ValueError("linear_mxfp4: gelu and residual exclude each other")
+        dtype, epi, ldr = torch.float32, _lib.EPI_BIAS_RESID_F32, _rows2d("linear_mxfp4: residual", residual, (torch.float32,))
         if residual.shape != (M, N):
             raise ValueError(f"linear_mxfp4: residual {tuple(residual.shape)} for a result of {(M, N)}")
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=x.device)
+        out, ldo = torch.empty((M, N), dtype=dtype, device=xt.device), N
     else:
-        _rows2d("linear_mxfp4: out", out, (dtype,))
+        ldo = _rows2d("linear_mxfp4: out", out, (dtype,))
         if out.shape != (M, N):
             raise ValueError(f"linear_mxfp4: out {tuple(out.shape)} for a result of {(M, N)}")
         same = residual is not None and out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()
-        _apart("linear_mxfp4", out, None if quantised else x, bias, None if same else residual, w.codes, w.scales,
-               x.codes if quantised else None, x.scales if quantised else None)
-    xc = x.codes if quantised else x
-    _same_device(xc, w.codes, bias, residual, out)
-    epi = _lib.EPI_BIAS_RESID_F32 if residual is not None else (_lib.EPI_BIAS_GELU_BF16 if gelu else _lib.EPI_BIAS_BF16)
-    tail = (M, N, K, epi, _ptr(bias), _ptr(residual), _ld(residual) if residual is not None else 0, out.data_ptr(), _ld(out))
+        _apart("linear_mxfp4", out, xt, bias, None if same else residual, w.data)
+    _same_device(xt, w.data, bias, residual, out)
+    wp, ws = w.pointers()
+    tail = (M, N, K, epi, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldo)
     if quantised:
-        _lib.check(lib.sgclip_mxfp4_gemm(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), *tail, _stream(xc)))
+        _lib.check(lib.sgclip_mxfp4_gemm(*x.pointers(), wp, ws, *tail, _stream(xt)))
         return out
     need = lib.sgclip_mxfp4_linear_workspace_bytes(M, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _lib.check(lib.sgclip_mxfp4_linear(x.data_ptr(), _lib.DTYPE_F32 if x.dtype == torch.float32 else _lib.DTYPE_BF16, _ld(x),
-                                       w.codes.data_ptr(), w.scales.data_ptr(), *tail, _ptr(ws), need, _stream(x)))
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.check(lib.sgclip_mxfp4_linear(x.data_ptr(), _MX_DTYPES[x.dtype], ldx, wp, ws, *tail, _ptr(scratch), need, _stream(x)))
     return out
 
 

@@ -507,15 +507,14 @@ class _LinearMxfp4Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(weight)
-        ctx.save_for_backward(xq.codes, xq.scales, wq.codes, wq.scales)
+        ctx.save_for_backward(xq.data, wq.data)
         ctx.shapes, ctx.dtypes = (xq.shape, wq.shape), (x.dtype, weight.dtype)
         return ops.linear_mxfp4(xq, wq, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xc, xs, wc, ws = ctx.saved_tensors
-        xq, wq = ops.Mxfp4(xc, xs, *ctx.shapes[0]), ops.Mxfp4(wc, ws, *ctx.shapes[1])
+        xq, wq = (ops.Mxfp4(data, *shape) for data, shape in zip(ctx.saved_tensors, ctx.shapes))
         dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, ctx.dtypes[0], *ctx.needs_input_grad)
         return dx, dw if dw is None else dw.to(ctx.dtypes[1]), db
 

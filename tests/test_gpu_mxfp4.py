@@ -180,7 +180,7 @@ def test_refusals():
                 lambda: ops.linear_mxfp4(x, w, residual=r, out=torch.empty(4, 9, device="cuda")),
                 lambda: ops.linear_mxfp4(x, w, residual=r, out=x[:, :8]),
                 lambda: ops.linear_mxfp4(x, w, residual=r[1:], out=r[:3]),
-                lambda: ops.Mxfp4(w.codes, w.scales, 8, 300), lambda: ops.Mxfp4(w.codes.float(), w.scales, 8, 64),
+                lambda: ops.Mxfp4(w.data, 8, 300), lambda: ops.Mxfp4(w.data.float(), 8, 64), lambda: ops.Mxfp4(w.data[1:], 8, 64),
                 lambda: training.linear_mxfp4(x, torch.randn(8, 63, device="cuda")),
                 lambda: G.linear_mxfp4_bwd(r, ops.quantize_mxfp4(x), ops.quantize_mxfp4(x))):
         with pytest.raises((ValueError, RuntimeError)):
@@ -222,6 +222,16 @@ def test_side_stream_and_replayed_graph():
         torch.cuda.synchronize()
         ea, ec, edx = step()
         assert torch.equal(a, ea) and torch.equal(c, ec) and torch.equal(dx, edx), k
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N", [(0, 5), (1, 1), (1, 512), (31, 513), (300, 77), (9000, 1032), (50, 8)])
+def test_column_sums(M, N, dtype):
+    x = _x(M, N + 3, dtype)[:, :N]
+    for v in (x, x.contiguous()):
+        got = G.column_sums(v)
+        _check(got, v.double().sum(0), v.double().abs().sum(0), M, 0)
+        assert torch.equal(G.column_sums(v), got)
 
 
 def _grads_64(x, w, dy):

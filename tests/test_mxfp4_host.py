@@ -24,6 +24,12 @@ def test_storage_sizes(lib):
     assert lib.sgclip_mxfp4_linear_workspace_bytes(17, 256) == 17 * 128 + 128 + 64 * 8   # codes rounded up to a multiple of 256, scales
 
 
+def test_python_storage_sizes_agree(lib):
+    for rows in (0, 1, 63, 64, 65, 1000, 1 << 20):
+        for cols in (1, 32, 255, 256, 257, 4096):
+            assert ops.Mxfp4.sizes(rows, cols) == (lib.sgclip_mxfp4_codes_bytes(rows, cols), lib.sgclip_mxfp4_scales_bytes(rows, cols))
+
+
 def test_entry_points_refuse_bad_arguments(lib):
     p = 4096  # an aligned address that no refused call touches
     E = _lib.EINVAL
@@ -54,7 +60,7 @@ def test_host_tensors_are_refused(lib):
     with pytest.raises(ValueError, match="GPU"):
         ops.quantize_mxfp4(torch.zeros(4, 32))
     with pytest.raises(ValueError):
-        ops.Mxfp4(torch.zeros(4 * 128, dtype=torch.uint8), torch.zeros(64 * 8, dtype=torch.uint8), 4, 32)
+        ops.Mxfp4(torch.zeros(4 * 128 + 64 * 8, dtype=torch.uint8), 4, 32)
     with pytest.raises(ValueError, match="fit"):
         training.linear_mxfp4(torch.zeros(4, 32), torch.zeros(8, 31))
 
