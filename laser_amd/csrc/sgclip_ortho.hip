@@ -5,8 +5,9 @@
 //   * every m x m product is computed on the tiles of one triangle and written to both;
 //   * several steps need X only once: M_i = p(A_i), Q <- M_i Q, A_{i+1} = M_i A_i M_i, then X <- Q X.  A block of k steps costs
 //     3 m^2 n + (4 k - 3) m^3 multiplications and additions instead of k (3 m^2 n + m^3).
-// The blocks are at most 3 steps long: squaring through A loses small singular values (the relative error of the result
-// grows from 1e-6 to 1e-5 at 3 steps and 7e-4 at 5, worst of the spectra tried, against 64 bits).
+// The price of a block is precision, since A holds the squares of the singular values: against 64 bits the result of five
+// steps is off by 1e-6 (relative, before its rounding) step by step and by 2e-5 to 1.5e-4 as one block, worst of gaussian, power-law,
+// exponential and low-rank spectra.  Blocks are at most five steps long, and only used where they save time.
 //
 // Precision.  The first steps multiply small singular values by a each, 485 times over five steps with the usual coefficients,
 // and rounding errors with them: with bf16 products the result is off by 2 to 20 %, with fp16 by 0.2 to 3 %.  Operands are
@@ -19,7 +20,8 @@
 #include "tile_common.h"
 
 #include <math.h>
-#include <stdlib.h>
+
+#include <type_traits>
 
 namespace sgclip {
 
@@ -90,14 +92,7 @@ __device__ __forceinline__ void or_store_rows(const f32x4 (&v)[SN], unsigned cha
 #pragma unroll
     for (int it0 = 0; it0 < 16 * SN * 4; it0 += 64) {
         const int it = it0 + lane, row = it / (SN * 4), w = it - row * (SN * 4);     // w: unit of 8 columns, hi / lo
-        int u, half;
-        if (SN % 2 == 0) {   // whole 32-column pieces: memory order
-            u = (w >> 3) * 4 + (w & 3);
-            half = (w >> 2) & 1;
-        } else {
-            u = w >> 1;
-            half = w & 1;
-        }
+        const int u = (w >> 3) * 4 + (w & 3), half = (w >> 2) & 1;   // memory order
         const int m = m0 + row, n = n0 + u * 8;
         if (m < M && n < npad) *(f16x8 *)(O + m * ld + or_unit(n) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
     }
@@ -125,31 +120,48 @@ __device__ __forceinline__ void or_store_cols(const f32x4 (&v)[SM], unsigned cha
 #pragma unroll
     for (int it0 = 0; it0 < 16 * SM * 4; it0 += 64) {
         const int it = it0 + lane, row = it / (SM * 4), w = it - row * (SM * 4);
-        int u, half;
-        if (SM % 2 == 0) {
-            u = (w >> 3) * 4 + (w & 3);
-            half = (w >> 2) & 1;
-        } else {
-            u = w >> 1;
-            half = w & 1;
-        }
+        const int u = (w >> 3) * 4 + (w & 3), half = (w >> 2) & 1;   // memory order
         const int n = n0 + row, m = m0 + u * 8;
         if (n < N && m < mpad) *(f16x8 *)(OT + n * ld + or_unit(m) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// WGM x WGN waves of 16 SM rows x 16 SN columns.  Two LDS slots of one 32-column stage each; per stage three products:
+// A wave's square block on the diagonal of a symmetric result, made exactly symmetric from its lower triangle.  What is left of
+// asymmetry grows from step to step (the error of five steps on one Gram matrix: 1e-5 with it, 1e-3 to 2e-2 without).
+template <int S>
+__device__ __forceinline__ void or_symmetrize(f32x4 (&v)[S][S], unsigned char *region, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    float *buf = (float *)region;
+#pragma unroll
+    for (int i = 0; i < S; i++)
+#pragma unroll
+        for (int j = 0; j <= i; j++) {
+            *(f32x4 *)(buf + r * 20 + q * 4) = v[i][j];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float t = buf[(q * 4 + e) * 20 + r];     // the element across the diagonal
+                if (i != j) v[j][i][e] = t;
+                else if (q * 4 + e > r) v[i][i][e] = t;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+}
+
+// 2 x 2 waves of 16 S rows x 16 S columns.  SLOTS LDS slots of one 32-column stage each; per stage three products:
 //   hi hi (reading the lo fragments of R), hi lo (reading those of L), then the stage's one barrier - every wave holds all
 //   of the stage in registers, the next stage has landed - and lo hi, during which the next stage's hi fragments are read and
-//   the DMA of the stage after it runs into the slot just freed.
-template <int EPI, int WGM, int WGN, int SM, int SN>
-__global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
-    constexpr int W = WGM * WGN, T = WGM * SM * 16, OP = T * 128, PIECES = T / 8 / W;
-    static_assert(T == WGN * SN * 16 && PIECES * W * 8 == T, "square tiles, whole pieces per wave");
+//   the DMA of stage s + SLOTS runs into the slot just freed.
+// S = 4 with two slots: two workgroups per CU, which is bound by the matrix pipe (24 of 1024 x 4096: 1.05 PFLOP/s of fp16
+// products on the products with K or N = 4096, 0.85 on the square ones, whose results cost as much traffic).
+// S = 2 with four slots, for few tiles, where a stage is shorter than its fetch.
+template <int EPI, int S, int SLOTS>
+__global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
+    constexpr int W = 4, T = 2 * S * 16, OP = T * 128, PIECES = T / 8 / W;
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WGN, wn = wave % WGN, r = lane & 15, q = lane >> 4;
+    const int wm = wave >> 1, wn = wave & 1, r = lane & 15, q = lane >> 4;
     constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
     const int per = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
     const int swz = xcd_remap(blockIdx.x, gridDim.x);
@@ -177,7 +189,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
     const unsigned char *lbase = (z ? g.L[1] : g.L[0]) + b * g.sL + m0 * ld, *rbase = g.R + b * g.sR + n0 * ld;
     const unsigned slots = (unsigned)(uintptr_t)LDS_PTR(lds) + wave * 1024;
     auto fetch = [&](int s) {
-        const unsigned slot = slots + (s & 1) * (2 * OP);
+        const unsigned slot = slots + (s & (SLOTS - 1)) * (2 * OP);
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
             p64_dma16(lbase, voff, p * step, maxl, slot + p * (W * 1024));
@@ -186,73 +198,89 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
         lbase += 128;
         rbase += 128;
     };
-    f32x4 acc[SM][SN];
+    f32x4 acc[S][S];
 #pragma unroll
-    for (int i = 0; i < SM; i++)
+    for (int i = 0; i < S; i++)
 #pragma unroll
-        for (int j = 0; j < SN; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < S; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     // lds_off of a row 16 further is 2048 bytes further, with the same chunk order
-    const int lh0 = lds_off(wm * SM * 16 + r, q), ll0 = lds_off(wm * SM * 16 + r, 4 + q);
-    const int rh0 = OP + lds_off(wn * SN * 16 + r, q), rl0 = OP + lds_off(wn * SN * 16 + r, 4 + q);
-    f16x8 lh[SM], ll[SM], rh[SN], rl[SN], rn[SN];
-    fetch(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (g.kc > 1) fetch(1);
-#pragma unroll
-    for (int i = 0; i < SM; i++) lh[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
-#pragma unroll
-    for (int j = 0; j < SN; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
-    for (int s = 0; s < g.kc; s++) {
-        const unsigned char *cur = lds + (s & 1) * (2 * OP), *nxt = lds + ((s + 1) & 1) * (2 * OP);
-        // R first: a lane's four results are four consecutive columns of one row
-#pragma unroll
-        for (int j = 0; j < SN; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
-#pragma unroll
-        for (int i = 0; i < SM; i++)
-#pragma unroll
-            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < SM; i++) ll[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
-#pragma unroll
-        for (int i = 0; i < SM; i++)
-#pragma unroll
-            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int p = 0; p < SM + SN; p++) {
-            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
-        }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const int lh0 = lds_off(wm * S * 16 + r, q), ll0 = lds_off(wm * S * 16 + r, 4 + q);
+    const int rh0 = OP + lds_off(wn * S * 16 + r, q), rl0 = OP + lds_off(wn * S * 16 + r, 4 + q);
+    f16x8 lh[S], ll[S], rh[S], rl[S], rn[S];
+    static_assert((SLOTS & (SLOTS - 1)) == 0 && (SLOTS - 1) * 2 * PIECES < 64, "slots by mask, outstanding fetches within the counter");
+    // Waits until the stage has landed after which `newer` stages were fetched (all of them in whole, or: everything), for all
+    // waves, with this wave's LDS reads done.
+    auto landed = [&](auto newer, bool whole) {
+        if (whole) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(newer)::value * 2 * PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 2 < g.kc) fetch(s + 2);
+    };
+    // at stage s, stages up to s + SLOTS - 1 have been fetched as far as there are that many
+    auto next_landed = [&](int s) { landed(std::integral_constant<int, SLOTS - 2>{}, s + SLOTS <= g.kc); };
+    for (int s = 0; s < min(SLOTS, g.kc); s++) fetch(s);
+    landed(std::integral_constant<int, SLOTS - 1>{}, SLOTS <= g.kc);
+#pragma unroll
+    for (int i = 0; i < S; i++) lh[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
+#pragma unroll
+    for (int j = 0; j < S; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
+    // a diagonal tile's wave above the diagonal only fetches: its block is written from below
+    const bool idle = SYM && ti == tj && wm < wn;
+    if (idle) {
+        for (int s = 0; s < g.kc; s++) {
+            next_landed(s);
+            if (s + SLOTS < g.kc) fetch(s + SLOTS);
+        }
+        __builtin_amdgcn_s_barrier();      // the one before the staging of the results
+        return;
+    }
+    for (int s = 0; s < g.kc; s++) {
+        const unsigned char *cur = lds + (s & (SLOTS - 1)) * (2 * OP), *nxt = lds + ((s + 1) & (SLOTS - 1)) * (2 * OP);
+        // R first: a lane's four results are four consecutive columns of one row
+#pragma unroll
+        for (int j = 0; j < S; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+#pragma unroll
+        for (int i = 0; i < S; i++)
+#pragma unroll
+            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < S; i++) ll[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
+#pragma unroll
+        for (int i = 0; i < S; i++)
+#pragma unroll
+            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < 2 * S; p++) {
+            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+        }
+        next_landed(s);
+        if (s + SLOTS < g.kc) fetch(s + SLOTS);
         // behind the last stage these read what the slot held before: not used
 #pragma unroll
-        for (int i = 0; i < SM; i++) lh[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
+        for (int i = 0; i < S; i++) lh[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
 #pragma unroll
-        for (int j = 0; j < SN; j++) rn[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
+        for (int j = 0; j < S; j++) rn[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
 #pragma unroll
-        for (int i = 0; i < SM; i++)
+        for (int i = 0; i < S; i++)
 #pragma unroll
-            for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
 #pragma unroll
-        for (int p = 0; p < SM + SN; p++) {
+        for (int p = 0; p < 2 * S; p++) {
             __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
             __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
         }
 #pragma unroll
-        for (int j = 0; j < SN; j++) rh[j] = rn[j];
+        for (int j = 0; j < S; j++) rh[j] = rn[j];
     }
 
     const float alpha = z ? g.alpha[1] : g.alpha[0];
-    const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16;
+    const int mw = m0 + wm * S * 16, nw = n0 + wn * S * 16;
     if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
 #pragma unroll
-        for (int i = 0; i < SM; i++)
+        for (int i = 0; i < S; i++)
 #pragma unroll
-            for (int j = 0; j < SN; j++) {
+            for (int j = 0; j < S; j++) {
                 const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
                 if (m >= g.M || n >= g.N) continue;
                 const f32x4 v = acc[i][j];
@@ -289,9 +317,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
         unsigned char *O = (z ? g.O[1] : g.O[0]) + b * g.sO;
         const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
 #pragma unroll
-        for (int i = 0; i < SM; i++)
+        for (int i = 0; i < S; i++)
 #pragma unroll
-            for (int j = 0; j < SN; j++) {
+            for (int j = 0; j < S; j++) {
                 if constexpr (EPI == OR_POLY) {
                     const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
                     f16x4 ah = {0, 0, 0, 0}, al = ah;
@@ -312,18 +340,19 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void or_gemm_kernel(OrGemm g) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        unsigned char *region = lds + wave * (4 * OP / W);
-        static_assert(16 * (SM * 64 + 16) <= 4 * OP / W && 16 * (SN * 64 + 16) <= 4 * OP / W, "a wave's staging fits its share of the LDS");
+        unsigned char *region = lds + wave * (SLOTS * 2 * OP / W);
+        static_assert(16 * (S * 64 + 16) <= SLOTS * 2 * OP / W && 16 * 20 * 4 <= SLOTS * 2 * OP / W, "a wave's staging fits its share of the LDS");
+        if (SYM && ti == tj && wm == wn) or_symmetrize<S>(acc, region, lane);
 #pragma unroll
-        for (int i = 0; i < SM; i++) or_store_rows<SN>(acc[i], region, O, ldn, mw + i * 16, nw, g.M, g.N, lane);
-        if (EPI == OR_BOTH || ti != tj) {
+        for (int i = 0; i < S; i++) or_store_rows<S>(acc[i], region, O, ldn, mw + i * 16, nw, g.M, g.N, lane);
+        if (EPI == OR_BOTH || ti != tj || wm != wn) {
             unsigned char *OT = EPI == OR_BOTH ? g.OT + b * g.sOT : O;
 #pragma unroll
-            for (int j = 0; j < SN; j++) {
-                f32x4 col[SM];
+            for (int j = 0; j < S; j++) {
+                f32x4 col[S];
 #pragma unroll
-                for (int i = 0; i < SM; i++) col[i] = acc[i][j];
-                or_store_cols<SM>(col, region, OT, ldm, mw, nw + j * 16, g.M, g.N, lane);
+                for (int i = 0; i < S; i++) col[i] = acc[i][j];
+                or_store_cols<S>(col, region, OT, ldm, mw, nw + j * 16, g.M, g.N, lane);
             }
         }
     }
@@ -363,6 +392,7 @@ __global__ __launch_bounds__(256) void or_norm_kernel(OrInput a, double *__restr
     double s = 0.0;
     const int step = a.vec ? 4 : 1, per = a.cols / step;
     const long long total = (long long)a.rows * per;
+#pragma unroll 4
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256 * OR_PARTS) {
         const long long row = i / per;
         const int col = (int)(i - row * per) * step;
@@ -512,8 +542,8 @@ struct OrSchedule {
 
 static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSchedule &o) {
     o.steps = steps;
-    // square matrices: blocks save nothing, single steps lose least
-    const int most = n * 4LL < m * 5LL ? 1 : 3;
+    // blocks save nothing for square matrices, and next to nothing where the launches' latency counts; single steps lose least
+    const int most = n * 4LL < m * 5LL || m < 256 ? 1 : 5;
     o.blocks = (steps + most - 1) / most;
     for (int i = 0; i < o.blocks; i++) o.len[i] = steps / o.blocks + (i < steps % o.blocks);
     double top = 1.0, qb = 1.0;     // bounds of the singular values (1 after the normalisation) and of Q
@@ -542,11 +572,11 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
     return or_exponent(top, o.ex[o.blocks]);
 }
 
-template <int EPI, int WGM, int WGN, int SM, int SN>
+template <int EPI, int S, int SLOTS>
 static int or_launch_tile(const OrGemm &g, long long blocks, int products, hipStream_t stream) {
-    constexpr int LDS = 4 * WGM * SM * 16 * 128;
-    if (!lds_attr((const void *)or_gemm_kernel<EPI, WGM, WGN, SM, SN>, LDS)) return SGCLIP_ELAUNCH;
-    or_gemm_kernel<EPI, WGM, WGN, SM, SN><<<dim3((unsigned)blocks, 1, products), 64 * WGM * WGN, LDS, stream>>>(g);
+    constexpr int LDS = SLOTS * 2 * (2 * S * 16) * 128;
+    if (!lds_attr((const void *)or_gemm_kernel<EPI, S, SLOTS>, LDS)) return SGCLIP_ELAUNCH;
+    or_gemm_kernel<EPI, S, SLOTS><<<dim3((unsigned)blocks, 1, products), 256, LDS, stream>>>(g);
     return launch_check("sgclip_orthogonalize");
 }
 
@@ -563,13 +593,10 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
         set_error("sgclip_orthogonalize: %d matrices of %d x %d are more than one launch holds", batch, g.M, g.N);
         return SGCLIP_EINVAL;
     }
-    const int cus = device_cus();
-    static const int force = getenv("OR_TILE") ? atoi(getenv("OR_TILE")) : 0;
-    if (force == 256) return or_launch_tile<EPI, 2, 4, 8, 4>(g, tiles(256), products, stream);
-    if (force == 192) return or_launch_tile<EPI, 2, 4, 6, 3>(g, tiles(192), products, stream);
-    if (force == 128) return or_launch_tile<EPI, 2, 2, 4, 4>(g, tiles(128), products, stream);
-    if (tiles(128) * products >= cus) return or_launch_tile<EPI, 2, 2, 4, 4>(g, tiles(128), products, stream);
-    return or_launch_tile<EPI, 2, 2, 2, 2>(g, tiles(64), products, stream);
+    // 128 x 128 tiles where they fill the chip, 64 x 64 below that (two of 127 x 255: 104 us, with 128 x 128 151 us).  192 and 256
+    // with eight waves measured 9 and 11 % slower on 24 of 1024 x 4096: fewer, larger tiles, and no second workgroup on the CU.
+    if (tiles(128) * products >= device_cus()) return or_launch_tile<EPI, 4, 2>(g, tiles(128), products, stream);
+    return or_launch_tile<EPI, 2, 4>(g, tiles(64), products, stream);
 }
 
 static inline float or_pow2(int e) { return ldexpf(1.0f, e); }
