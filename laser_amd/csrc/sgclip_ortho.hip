@@ -549,6 +549,7 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
     double top = 1.0, qb = 1.0;     // bounds of the singular values (1 after the normalisation) and of Q
     for (int k = 0, blk = 0, in = 0; k < steps; k++) {
         const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+        if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
         o.s[k].a = a;
         o.s[k].b = b;
         o.s[k].c = c;
@@ -560,7 +561,7 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
             tm = fmax(tm, t * p);
             next = fmax(next, s * p);
         }
-        if (!(pm == pm) || !or_exponent(pm, o.s[k].em) || !or_exponent(tm, o.s[k].et) || !or_exponent(next * next, o.s[k].ea)) return false;
+        if (!or_exponent(pm, o.s[k].em) || !or_exponent(tm, o.s[k].et) || !or_exponent(next * next, o.s[k].ea)) return false;
         qb = in == 0 ? pm : qb * pm;
         if (!or_exponent(qb, o.eq[k])) return false;
         top = next;

@@ -350,27 +350,38 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, e
     return out
 
 
-def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], lr: float, momentum: float = 0.95,
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta, lr: float, momentum: float = 0.95,
               nesterov: bool = True, weight_decay: float = 0.0, scale: float = 1.0, steps: int = 5, coefficients=NEWTON_SCHULZ,
               eps: float = 1e-7):
     """One orthogonalised-momentum step on matrices of one shape (contiguous f32 [rows, cols] each), in place:
     m = momentum m + (1 - momentum) g; u = (1 - momentum) g + momentum m (nesterov) or m;
-    p = (1 - lr weight_decay) p - lr scale orthogonalize(u).  The matrices of a call share its launches."""
-    if not len(params) == len(grads) == len(momenta):
-        raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
-    if not params:
+    p = (1 - lr weight_decay) p - lr scale orthogonalize(u).  momenta: a list like the others, or one tensor [count, rows, cols].
+    The matrices of a call share its launches."""
+    n = len(params)
+    if not n == len(grads) == len(momenta):
+        raise ValueError(f"muon_step: {n} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    if n == 0:
         return
     shape, dev = params[0].shape, params[0].device
     if len(shape) != 2 or dev.type != "cuda":
         raise ValueError(f"muon_step: expected matrices on the GPU, got {tuple(shape)} on {dev}")
-    for t in (*params, *grads, *momenta):
-        if t.dtype != F32 or t.shape != shape or t.device != dev or not t.is_contiguous():
+    stacked = isinstance(momenta, torch.Tensor)
+    for t in (*params, *grads, *((momenta,) if stacked else momenta)):
+        if t.dtype != F32 or t.shape != ((n, *shape) if t is momenta else shape) or t.device != dev or not t.is_contiguous():
             raise ValueError(f"muon_step: every tensor must be contiguous f32 {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if len({t.data_ptr() for t in (*params, *momenta)}) != 2 * len(params):
-        raise ValueError("muon_step: a parameter or momentum occurs twice")
+    size = 4 * shape[0] * shape[1]
+    at = [[t.data_ptr() for t in params], [t.data_ptr() for t in grads],
+          range(momenta.data_ptr(), momenta.data_ptr() + n * size, size) if stacked else [t.data_ptr() for t in momenta]]
+    if size == 0:
+        return
+    # what is written must not lie in anything else that is read or written
+    spans = sorted([(p, True) for p in at[0]] + [(p, False) for p in set(at[1])] + [(p, True) for p in at[2]])
+    for (a, wa), (b, wb) in zip(spans, spans[1:]):
+        if b < a + size and (wa or wb):
+            raise ValueError("muon_step: parameters, gradients and momenta overlap, or one occurs twice")
     table = _coefficients(coefficients, steps)
-    lib, n = _lib.load(), len(params)
-    tables = [(C.c_void_p * n)(*(t.data_ptr() for t in ts)) for ts in (params, grads, momenta)]
+    lib = _lib.load()
+    tables = [(C.c_void_p * n)(*ps) for ps in at]
     need = lib.sgclip_orthogonalize_workspace_bytes(n, *shape)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.check(lib.sgclip_muon_step(*tables, n, shape[0], shape[1], momentum, 1 if nesterov else 0, lr, weight_decay, scale, table, steps, eps,

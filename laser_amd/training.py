@@ -532,7 +532,11 @@ def linear_mxfp4(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         # autograd's own bookkeeping of the leaves may belong to another stream, which a capture does not survive
         raise RuntimeError("linear_mxfp4 builds no autograd graph under graph capture: call ops.linear_mxfp4 and "
                            "grad_ops.linear_mxfp4_bwd")
-    y = _LinearMxfp4Fn.apply(x.reshape(-1, x.shape[-1]).contiguous(), weight.contiguous(), bias)
+    if weight.stride(1) != 1 or not x.is_contiguous():
+        x, weight = x.contiguous(), weight.contiguous()
+    if x.dim() == 2:
+        return _LinearMxfp4Fn.apply(x, weight, bias)
+    y = _LinearMxfp4Fn.apply(x.reshape(-1, x.shape[-1]), weight, bias)
     return y.view(x.shape[:-1] + (weight.shape[0],))
 
 
@@ -640,8 +644,9 @@ class Muon:
             rows, cols = group[0].shape
             scale = 0.2 * max(rows, cols) ** 0.5 if self.adjust == "rms" else max(1.0, rows / cols) ** 0.5
             params = [group[i] for i in at]
-            G.muon_step([p.data for p in params], [p.grad.to(F32).contiguous() for p in params], [buf[i] for i in at], self.lr, self.beta,
-                        self.nesterov, self.weight_decay, scale, self.steps, self.coefficients, self.eps)
+            grads = [p.grad if p.grad.dtype == F32 and p.grad.is_contiguous() else p.grad.to(F32).contiguous() for p in params]
+            G.muon_step(params, grads, buf if len(at) == len(group) else [buf[i] for i in at], self.lr, self.beta, self.nesterov,
+                        self.weight_decay, scale, self.steps, self.coefficients, self.eps)
             for p in params:
                 torch.autograd.graph.increment_version(p)   # the towers rebuild their bf16 copies when this changes
 
