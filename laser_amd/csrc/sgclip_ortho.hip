@@ -53,12 +53,12 @@ struct OrGemm {
     unsigned char *O[2];               // split rows [M][N], or with OR_BOTH also
     unsigned char *OT;                 // their transpose [N][M]
     const unsigned char *A;            // OR_POLY: A's split rows
-    long long sL, sR, sO, sOT;         // bytes from one matrix of the batch to the next
-    float alpha[2];                    // power of two from the accumulator's scale to the output's
-    float ca, cb, cc;                  // OR_POLY: out = ca I + cb A + cc (A A)
+    long long sL, sR, sO, sOT, sA;     // bytes from one matrix of the batch to the next
+    float alpha[2];                    // from the accumulator's scale to the output's
+    float ca, cb;                      // OR_POLY: out = alpha (ca I + cb A + A A), the first two in the accumulators from the start
     float decay, rate;                 // OR_UPDATE: p = decay p - rate out
     long long ldo;                     // OR_OUT / OR_UPDATE: row stride in elements
-    int M, N, kc;                      // rows of L, rows of R, 32-column pieces of both
+    int M, N, kc, ldk;                 // rows of L, rows of R, 32-column pieces of both to walk (0: none), bytes of their rows
     int tiles_m, tiles_n, wide;
     OrPointers out;                    // OR_OUT: bf16, OR_UPDATE: f32 parameters
 };
@@ -67,10 +67,11 @@ struct OrGemm {
 // Items of a row in memory order: per 32 columns four 16-byte units of hi, then four of lo.
 __device__ __forceinline__ long long or_unit(int col) { return (long long)(col >> 5) * 128 + (col & 31) * 2; }
 
-// v: the wave's results for 16 rows (m0 ..) x 16 SN columns (n0 ..); columns at or behind N are zeros in the padding.
+// v: the wave's results for 16 rows (m0 ..) x 16 SN columns (n0 ..); columns at or behind N are zeros in the padding.  lower: only the
+// 16 x 16 blocks on and below the diagonal.
 template <int SN>
 __device__ __forceinline__ void or_store_rows(const f32x4 (&v)[SN], unsigned char *region, unsigned char *O, long long ld, int m0, int n0, int M,
-                                              int N, int lane) {
+                                              int N, bool lower, int lane) {
     constexpr int RS = SN * 64 + 16;     // bytes of a staged row: 16 SN columns x 4, and 16 against bank conflicts
     const int r = lane & 15, q = lane >> 4;
 #pragma unroll
@@ -92,17 +93,17 @@ __device__ __forceinline__ void or_store_rows(const f32x4 (&v)[SN], unsigned cha
 #pragma unroll
     for (int it0 = 0; it0 < 16 * SN * 4; it0 += 64) {
         const int it = it0 + lane, row = it / (SN * 4), w = it - row * (SN * 4);     // w: unit of 8 columns, hi / lo
-        const int u = (w >> 3) * 4 + (w & 3), half = (w >> 2) & 1;   // memory order
+        const int u = SN % 2 ? w >> 1 : (w >> 3) * 4 + (w & 3), half = SN % 2 ? w & 1 : (w >> 2) & 1;   // in memory order for whole pieces
         const int m = m0 + row, n = n0 + u * 8;
-        if (m < M && n < npad) *(f16x8 *)(O + m * ld + or_unit(n) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
+        if (m < M && n < npad && !(lower && (n >> 4) > (m >> 4))) *(f16x8 *)(O + m * ld + or_unit(n) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// The transpose: 16 columns (n0 ..) of the wave's 16 SM rows (m0 ..) become 16 rows of OT.
+// The transpose: 16 columns (n0 ..) of the wave's 16 SM rows (m0 ..) become 16 rows of OT; lower: only what lies below the diagonal.
 template <int SM>
 __device__ __forceinline__ void or_store_cols(const f32x4 (&v)[SM], unsigned char *region, unsigned char *OT, long long ld, int m0, int n0, int M,
-                                              int N, int lane) {
+                                              int N, bool lower, int lane) {
     constexpr int RS = SM * 64 + 16;
     const int r = lane & 15, q = lane >> 4;
 #pragma unroll
@@ -120,48 +121,42 @@ __device__ __forceinline__ void or_store_cols(const f32x4 (&v)[SM], unsigned cha
 #pragma unroll
     for (int it0 = 0; it0 < 16 * SM * 4; it0 += 64) {
         const int it = it0 + lane, row = it / (SM * 4), w = it - row * (SM * 4);
-        const int u = (w >> 3) * 4 + (w & 3), half = (w >> 2) & 1;   // memory order
+        const int u = SM % 2 ? w >> 1 : (w >> 3) * 4 + (w & 3), half = SM % 2 ? w & 1 : (w >> 2) & 1;   // in memory order for whole pieces
         const int n = n0 + row, m = m0 + u * 8;
-        if (n < N && m < mpad) *(f16x8 *)(OT + n * ld + or_unit(m) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
+        if (n < N && m < mpad && !(lower && (m >> 4) <= (n >> 4))) *(f16x8 *)(OT + n * ld + or_unit(m) + half * 64) = *(const f16x8 *)(region + row * RS + u * 32 + half * 16);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// A wave's square block on the diagonal of a symmetric result, made exactly symmetric from its lower triangle.  What is left of
+// A 16 x 16 block on the diagonal of a symmetric result, made exactly symmetric from its lower triangle.  What is left of
 // asymmetry grows from step to step (the error of five steps on one Gram matrix: 1e-5 with it, 1e-3 to 2e-2 without).
-template <int S>
-__device__ __forceinline__ void or_symmetrize(f32x4 (&v)[S][S], unsigned char *region, int lane) {
+__device__ __forceinline__ void or_symmetrize(f32x4 &v, unsigned char *region, int lane) {
     const int r = lane & 15, q = lane >> 4;
     float *buf = (float *)region;
+    *(f32x4 *)(buf + r * 20 + q * 4) = v;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < S; i++)
-#pragma unroll
-        for (int j = 0; j <= i; j++) {
-            *(f32x4 *)(buf + r * 20 + q * 4) = v[i][j];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float t = buf[(q * 4 + e) * 20 + r];     // the element across the diagonal
-                if (i != j) v[j][i][e] = t;
-                else if (q * 4 + e > r) v[i][i][e] = t;
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
+    for (int e = 0; e < 4; e++) {
+        const float t = buf[(q * 4 + e) * 20 + r];     // the element across the diagonal
+        if (q * 4 + e > r) v[e] = t;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// 2 x 2 waves of 16 S rows x 16 S columns.  SLOTS LDS slots of one 32-column stage each; per stage three products:
-//   hi hi (reading the lo fragments of R), hi lo (reading those of L), then the stage's one barrier - every wave holds all
-//   of the stage in registers, the next stage has landed - and lo hi, during which the next stage's hi fragments are read and
-//   the DMA of stage s + SLOTS runs into the slot just freed.
-// S = 4 with two slots: two workgroups per CU, which is bound by the matrix pipe (24 of 1024 x 4096: 1.05 PFLOP/s of fp16
-// products on the products with K or N = 4096, 0.85 on the square ones, whose results cost as much traffic).
-// S = 2 with four slots, for few tiles, where a stage is shorter than its fetch.
-template <int EPI, int S, int SLOTS>
-__global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
-    constexpr int W = 4, T = 2 * S * 16, OP = T * 128, PIECES = T / 8 / W;
+// WM x WN waves of 16 SM rows x 16 SN columns.  SLOTS LDS slots of one 32-column stage each; per stage three products, hi hi, hi lo and
+// lo hi (of L and R).  Fragments roll through one set of registers: those of L arrive a few products before their use and are
+// replaced, hi by lo, row by row; in the middle of the last product every wave holds the rest of the stage, the next stage has
+// landed (the one barrier), and the DMA of stage s + SLOTS starts into the slot just freed.
+//   256 x 256: eight waves, 243 registers, 16.1 results per cycle and CU of 21.3 the matrix pipe could do;
+//   192 x 192: eight waves, three slots; 128 x 128: four waves, two workgroups on a CU; both spend 89 - 100 % of the LDS's cycles;
+//   64 x 64: four waves, four slots, for few tiles, where a stage is shorter than its fetch.
+template <int EPI, int WM, int WN, int SM, int SN, int SLOTS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
+    constexpr int W = WM * WN, T = WM * SM * 16, OP = T * 128, PIECES = T / 8 / W, SLOT = 2 * OP;
+    static_assert(T == WN * SN * 16 && PIECES * W * 8 == T, "square tiles, whole pieces per wave");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1, r = lane & 15, q = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN, r = lane & 15, q = lane >> 4;
     constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
     const int per = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
     const int swz = xcd_remap(blockIdx.x, gridDim.x);
@@ -179,7 +174,7 @@ __global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
     ti = __builtin_amdgcn_readfirstlane(ti);
     tj = __builtin_amdgcn_readfirstlane(tj);
     const int m0 = ti * T, n0 = tj * T;
-    const long long ld = (long long)g.kc * 128;
+    const long long ld = (long long)g.ldk, ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
 
     // DMA of a stage: the wave's pieces of 8 rows, wave + W p, rows behind the matrix clamped to its last one
     const int prow = wave * 8 + (lane >> 3);
@@ -188,26 +183,33 @@ __global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
     const unsigned maxl = (unsigned)(min(g.M - 1 - m0, T - 1) * ld) + chunk, maxr = (unsigned)(min(g.N - 1 - n0, T - 1) * ld) + chunk;
     const unsigned char *lbase = (z ? g.L[1] : g.L[0]) + b * g.sL + m0 * ld, *rbase = g.R + b * g.sR + n0 * ld;
     const unsigned slots = (unsigned)(uintptr_t)LDS_PTR(lds) + wave * 1024;
-    auto fetch = [&](int s) {
-        const unsigned slot = slots + (s & (SLOTS - 1)) * (2 * OP);
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-            p64_dma16(lbase, voff, p * step, maxl, slot + p * (W * 1024));
-            p64_dma16(rbase, voff, p * step, maxr, slot + OP + p * (W * 1024));
-        }
-        lbase += 128;
-        rbase += 128;
+    // piece p of the next stage to fetch: the wave's PIECES of L, then of R
+    auto fetch_piece = [&](unsigned slot, int p) {
+        if (p < PIECES) p64_dma16(lbase, voff, p * step, maxl, slot + p * (W * 1024));
+        else p64_dma16(rbase, voff, (p - PIECES) * step, maxr, slot + OP + (p - PIECES) * (W * 1024));
     };
-    f32x4 acc[S][S];
+    const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16;
+    f32x4 acc[SM][SN];
 #pragma unroll
-    for (int i = 0; i < S; i++)
+    for (int i = 0; i < SM; i++)
 #pragma unroll
-        for (int j = 0; j < S; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < SN; j++) {
+            acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if constexpr (EPI == OR_POLY) {
+                const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
+                if (m < g.M && n < or_chunks(g.N) * 32) {
+                    const unsigned char *a = g.A + b * g.sA + m * ldn + or_unit(n);
+                    const f16x4 ah = *(const f16x4 *)a, al = *(const f16x4 *)(a + 64);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
+                }
+            }
+        }
     // lds_off of a row 16 further is 2048 bytes further, with the same chunk order
-    const int lh0 = lds_off(wm * S * 16 + r, q), ll0 = lds_off(wm * S * 16 + r, 4 + q);
-    const int rh0 = OP + lds_off(wn * S * 16 + r, q), rl0 = OP + lds_off(wn * S * 16 + r, 4 + q);
-    f16x8 lh[S], ll[S], rh[S], rl[S], rn[S];
-    static_assert((SLOTS & (SLOTS - 1)) == 0 && (SLOTS - 1) * 2 * PIECES < 64, "slots by mask, outstanding fetches within the counter");
+    const int lh0 = lds_off(wm * SM * 16 + r, q), ll0 = lds_off(wm * SM * 16 + r, 4 + q);
+    const int rh0 = OP + lds_off(wn * SN * 16 + r, q), rl0 = OP + lds_off(wn * SN * 16 + r, 4 + q);
+    f16x8 l[SM], rh[SN], rl[SN];
+    static_assert(SLOTS >= 2 && (SLOTS - 1) * 2 * PIECES < 64, "outstanding fetches within the counter");
     // Waits until the stage has landed after which `newer` stages were fetched (all of them in whole, or: everything), for all
     // waves, with this wave's LDS reads done.
     auto landed = [&](auto newer, bool whole) {
@@ -218,69 +220,85 @@ __global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
     };
     // at stage s, stages up to s + SLOTS - 1 have been fetched as far as there are that many
     auto next_landed = [&](int s) { landed(std::integral_constant<int, SLOTS - 2>{}, s + SLOTS <= g.kc); };
-    for (int s = 0; s < min(SLOTS, g.kc); s++) fetch(s);
+    auto fetch = [&](int slot) {
+#pragma unroll
+        for (int p = 0; p < 2 * PIECES; p++) fetch_piece(slots + slot, p);
+        lbase += 128;
+        rbase += 128;
+    };
+    for (int s = 0; s < min(SLOTS, g.kc); s++) fetch(s * SLOT);
     landed(std::integral_constant<int, SLOTS - 1>{}, SLOTS <= g.kc);
+    constexpr int H = SM / 2;
 #pragma unroll
-    for (int i = 0; i < S; i++) lh[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
+    for (int i = 0; i < H; i++) l[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
 #pragma unroll
-    for (int j = 0; j < S; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
+    for (int j = 0; j < SN; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
     // a diagonal tile's wave above the diagonal only fetches: its block is written from below
-    const bool idle = SYM && ti == tj && wm < wn;
-    if (idle) {
+    int slot = 0;
+    if (SYM && mw + SM * 16 <= nw) {
         for (int s = 0; s < g.kc; s++) {
             next_landed(s);
-            if (s + SLOTS < g.kc) fetch(s + SLOTS);
+            if (s + SLOTS < g.kc) fetch(slot);
+            slot = slot == (SLOTS - 1) * SLOT ? 0 : slot + SLOT;
         }
         __builtin_amdgcn_s_barrier();      // the one before the staging of the results
         return;
     }
-    for (int s = 0; s < g.kc; s++) {
-        const unsigned char *cur = lds + (s & (SLOTS - 1)) * (2 * OP), *nxt = lds + ((s + 1) & (SLOTS - 1)) * (2 * OP);
-        // R first: a lane's four results are four consecutive columns of one row
+    auto multiply = [&](int i, const f16x8(&rr)[SN]) {     // R first: a lane's four results are four consecutive columns of one row
 #pragma unroll
-        for (int j = 0; j < S; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+        for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rr[j], l[i], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto stage = [&](int s, auto fetching) {
+        const int next = slot == (SLOTS - 1) * SLOT ? 0 : slot + SLOT;
+        const unsigned char *cur = lds + slot, *nxt = lds + next;
 #pragma unroll
-        for (int i = 0; i < S; i++)
+        for (int i = 0; i < SM; i++) {          // hi hi; the rest of L's hi fragments and R's lo fragments arrive
+            if (i < SM - H) l[H + i] = *(const f16x8 *)(cur + lh0 + (H + i) * 2048);
 #pragma unroll
-            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], lh[i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < S; i++) ll[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
-#pragma unroll
-        for (int i = 0; i < S; i++)
-#pragma unroll
-            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[j], lh[i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int p = 0; p < 2 * S; p++) {
-            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+            for (int j = i * SN / SM; j < (i + 1) * SN / SM; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+            multiply(i, rh);
         }
+#pragma unroll
+        for (int i = 0; i < SM; i++) {          // hi lo; L's lo fragments take the places of the hi ones
+            multiply(i, rl);
+            l[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
+        }
+#pragma unroll
+        for (int i = 0; i < H; i++) multiply(i, rh);
         next_landed(s);
-        if (s + SLOTS < g.kc) fetch(s + SLOTS);
-        // behind the last stage these read what the slot held before: not used
+        // The fetches go out one by one between the products: in one burst a wave waits 16 cycles for each to be taken, and the
+        // matrix pipe with it.  Behind the last stage the reads return what the slot held before: not used.
+        constexpr int F = 2 * PIECES, G = SM - H;
 #pragma unroll
-        for (int i = 0; i < S; i++) lh[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
+        for (int i = 0; i < G; i++) {           // lo hi; half of the next stage's hi fragments arrive
+            if constexpr (decltype(fetching)::value) {
 #pragma unroll
-        for (int j = 0; j < S; j++) rn[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
+                for (int p = i * F / G; p < (i + 1) * F / G; p++) fetch_piece(slots + slot, p);
+            }
+            if (i < H) l[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
 #pragma unroll
-        for (int i = 0; i < S; i++)
-#pragma unroll
-            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[j], ll[i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int p = 0; p < 2 * S; p++) {
-            __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+            for (int j = i * SN / G; j < (i + 1) * SN / G; j++) rl[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
+            multiply(H + i, rh);
+        }
+        if constexpr (decltype(fetching)::value) {
+            lbase += 128;
+            rbase += 128;
         }
 #pragma unroll
-        for (int j = 0; j < S; j++) rh[j] = rn[j];
-    }
+        for (int j = 0; j < SN; j++) rh[j] = rl[j];
+        slot = next;
+    };
+    int s = 0;
+    for (; s + SLOTS < g.kc; s++) stage(s, std::true_type{});
+    for (; s < g.kc; s++) stage(s, std::false_type{});
 
     const float alpha = z ? g.alpha[1] : g.alpha[0];
-    const int mw = m0 + wm * S * 16, nw = n0 + wn * S * 16;
     if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
 #pragma unroll
-        for (int i = 0; i < S; i++)
+        for (int i = 0; i < SM; i++)
 #pragma unroll
-            for (int j = 0; j < S; j++) {
+            for (int j = 0; j < SN; j++) {
                 const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
                 if (m >= g.M || n >= g.N) continue;
                 const f32x4 v = acc[i][j];
@@ -315,45 +333,36 @@ __global__ __launch_bounds__(256, 2) void or_gemm_kernel(OrGemm g) {
             }
     } else {
         unsigned char *O = (z ? g.O[1] : g.O[0]) + b * g.sO;
-        const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
 #pragma unroll
-        for (int i = 0; i < S; i++)
+        for (int i = 0; i < SM; i++)
 #pragma unroll
-            for (int j = 0; j < S; j++) {
-                if constexpr (EPI == OR_POLY) {
-                    const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
-                    f16x4 ah = {0, 0, 0, 0}, al = ah;
-                    if (m < g.M && n < or_chunks(g.N) * 32) {
-                        const unsigned char *a = g.A + b * g.sL + m * ld + or_unit(n);
-                        ah = *(const f16x4 *)a;
-                        al = *(const f16x4 *)(a + 64);
-                    }
+            for (int j = 0; j < SN; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        acc[i][j][e] = g.cc * acc[i][j][e] + g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] *= alpha;
-                }
-            }
+                for (int e = 0; e < 4; e++) acc[i][j][e] *= alpha;
         // the last stage's unused reads are done with the LDS (lgkmcnt), every wave has passed its last barrier's reads
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        unsigned char *region = lds + wave * (SLOTS * 2 * OP / W);
-        static_assert(16 * (S * 64 + 16) <= SLOTS * 2 * OP / W && 16 * 20 * 4 <= SLOTS * 2 * OP / W, "a wave's staging fits its share of the LDS");
-        if (SYM && ti == tj && wm == wn) or_symmetrize<S>(acc, region, lane);
+        constexpr int REGION = SLOTS * SLOT / W / 16 * 16;
+        unsigned char *region = lds + wave * REGION;
+        static_assert(16 * (SM * 64 + 16) <= REGION && 16 * (SN * 64 + 16) <= REGION && 16 * 20 * 4 <= REGION, "a wave's staging fits its share of the LDS");
+        const bool diagonal = SYM && ti == tj;
+        if (diagonal) {
 #pragma unroll
-        for (int i = 0; i < S; i++) or_store_rows<S>(acc[i], region, O, ldn, mw + i * 16, nw, g.M, g.N, lane);
-        if (EPI == OR_BOTH || ti != tj || wm != wn) {
-            unsigned char *OT = EPI == OR_BOTH ? g.OT + b * g.sOT : O;
+            for (int i = 0; i < SM; i++)
 #pragma unroll
-            for (int j = 0; j < S; j++) {
-                f32x4 col[S];
+                for (int j = 0; j < SN; j++)
+                    if (mw + i * 16 == nw + j * 16) or_symmetrize(acc[i][j], region, lane);
+        }
 #pragma unroll
-                for (int i = 0; i < S; i++) col[i] = acc[i][j];
-                or_store_cols<S>(col, region, OT, ldm, mw, nw + j * 16, g.M, g.N, lane);
-            }
+        for (int i = 0; i < SM; i++) or_store_rows<SN>(acc[i], region, O, ldn, mw + i * 16, nw, g.M, g.N, diagonal, lane);
+        unsigned char *OT = EPI == OR_BOTH ? g.OT + b * g.sOT : O;
+#pragma unroll
+        for (int j = 0; j < SN; j++) {
+            f32x4 col[SM];
+#pragma unroll
+            for (int i = 0; i < SM; i++) col[i] = acc[i][j];
+            or_store_cols<SM>(col, region, OT, ldm, mw, nw + j * 16, g.M, g.N, diagonal, lane);
         }
     }
 }
@@ -573,11 +582,11 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
     return or_exponent(top, o.ex[o.blocks]);
 }
 
-template <int EPI, int S, int SLOTS>
+template <int EPI, int WM, int WN, int SM, int SN, int SLOTS>
 static int or_launch_tile(const OrGemm &g, long long blocks, int products, hipStream_t stream) {
-    constexpr int LDS = SLOTS * 2 * (2 * S * 16) * 128;
-    if (!lds_attr((const void *)or_gemm_kernel<EPI, S, SLOTS>, LDS)) return SGCLIP_ELAUNCH;
-    or_gemm_kernel<EPI, S, SLOTS><<<dim3((unsigned)blocks, 1, products), 256, LDS, stream>>>(g);
+    constexpr int LDS = SLOTS * 2 * (WM * SM * 16) * 128;
+    if (!lds_attr((const void *)or_gemm_kernel<EPI, WM, WN, SM, SN, SLOTS>, LDS)) return SGCLIP_ELAUNCH;
+    or_gemm_kernel<EPI, WM, WN, SM, SN, SLOTS><<<dim3((unsigned)blocks, 1, products), 64 * WM * WN, LDS, stream>>>(g);
     return launch_check("sgclip_orthogonalize");
 }
 
@@ -594,10 +603,17 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
         set_error("sgclip_orthogonalize: %d matrices of %d x %d are more than one launch holds", batch, g.M, g.N);
         return SGCLIP_EINVAL;
     }
-    // 128 x 128 tiles where they fill the chip, 64 x 64 below that (two of 127 x 255: 104 us, with 128 x 128 151 us).  192 and 256
-    // with eight waves measured 9 and 11 % slower on 24 of 1024 x 4096: fewer, larger tiles, and no second workgroup on the CU.
-    if (tiles(128) * products >= device_cus()) return or_launch_tile<EPI, 4, 2>(g, tiles(128), products, stream);
-    return or_launch_tile<EPI, 2, 4>(g, tiles(64), products, stream);
+    // 64 x 64 tiles where 128 x 128 do not give every CU one (two of 127 x 255: 104 us, with 128 x 128 151 us).  Otherwise the tile whose
+    // rounds over the chip cost least: cycles of a stage measured at 1024 x 4096 and 768 x 768, 4080 for a 256 x 256 tile, 2400 for
+    // 192 x 192, 2330 for two 128 x 128 tiles that share a CU (16.1, 15.4 and 14.1 results per cycle: the larger the tile, the less LDS
+    // traffic per product).  48 of 768 x 768: 192 where X is written (3 rounds), 128 on the triangles; 24 of 1024 x 4096: 256.
+    const int cus = device_cus();
+    if (tiles(128) * products < cus) return or_launch_tile<EPI, 2, 2, 2, 2, 4>(g, tiles(64), products, stream);
+    auto cost = [&](int T, int slots, int cycles) { return (tiles(T) * products + slots - 1) / slots * cycles; };
+    const long long c128 = cost(128, 2 * cus, 2330), c192 = cost(192, cus, 2400), c256 = cost(256, cus, 4080);
+    if (c256 <= c192 && c256 <= c128) return or_launch_tile<EPI, 2, 4, 8, 4, 2>(g, tiles(256), products, stream);
+    if (c192 < c128) return or_launch_tile<EPI, 2, 4, 6, 3, 3>(g, tiles(192), products, stream);
+    return or_launch_tile<EPI, 2, 2, 4, 4, 2>(g, tiles(128), products, stream);
 }
 
 static inline float or_pow2(int e) { return ldexpf(1.0f, e); }
@@ -625,10 +641,12 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
         g.sL = g.sR = (long long)p.x;
         g.sO = (long long)p.sq;
         g.kc = kn;
+        g.ldk = kn * 128;
         g.alpha[0] = or_pow2(ea - 2 * sch.ex[blk]);
         rc = or_launch<OR_SYM>(g, batch, 1, stream);
-        g.sL = g.sR = (long long)p.sq;
+        g.sL = g.sR = g.sA = (long long)p.sq;
         g.kc = km;
+        g.ldk = km * 128;
         for (int i = 0; i < sch.len[blk] && rc == SGCLIP_OK; i++, k++) {
             const OrStep &s = sch.s[k];
             const bool last = i + 1 == sch.len[blk];
@@ -636,10 +654,15 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
             g.L[0] = g.R = g.A = A;
             unsigned char *Mi = i == 0 ? Q : M;
             g.O[0] = Mi;
-            g.ca = (float)ldexp(s.a, s.em);
-            g.cb = (float)ldexp(s.b, s.em - ea);
-            g.cc = (float)ldexp(s.c, s.em - 2 * ea);
+            // a coefficient c below the rounding of the others' terms is none: then nothing is multiplied
+            const bool square = fabs(s.c) > 1e-12 * fmax(fabs(s.a), fabs(s.b));
+            const double c = square ? ldexp(s.c, s.em - 2 * ea) : 1.0;
+            g.alpha[0] = (float)c;
+            g.ca = (float)(ldexp(s.a, s.em) / c);
+            g.cb = (float)(ldexp(s.b, s.em - ea) / c);
+            g.kc = square ? km : 0;
             if ((rc = or_launch<OR_POLY>(g, batch, 1, stream)) != SGCLIP_OK) break;
+            g.kc = km;
             if (i == 0) eq = s.em;
             // T = A M and Q = Q M, whichever are needed
             int np = 0;
