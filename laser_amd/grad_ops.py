@@ -280,8 +280,8 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
     M, N, K = xq.rows, wq.rows, xq.cols
     dev = dy.device
     db = column_sums(dy) if need_db else None
-    if M == 0:
-        return (torch.empty((0, K), dtype=dx_dtype, device=dev) if need_dx else None,
+    if M == 0 or N == 0:
+        return (torch.zeros((M, K), dtype=dx_dtype, device=dev) if need_dx else None,
                 torch.zeros((N, K), dtype=F32, device=dev) if need_dw else None, db)
     dyb = cast_bf16(dy) if dy.dtype == F32 else dy
     dx = None

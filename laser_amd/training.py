@@ -514,6 +514,8 @@ class _LinearMxfp4Fn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("linear_mxfp4's backward is not captured: call grad_ops.linear_mxfp4_bwd")
         xq, wq = (ops.Mxfp4(data, *shape) for data, shape in zip(ctx.saved_tensors, ctx.shapes))
         dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, ctx.dtypes[0], *ctx.needs_input_grad)
         return dx, dw if dw is None else dw.to(ctx.dtypes[1]), db
@@ -532,8 +534,7 @@ def linear_mxfp4(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         # autograd's own bookkeeping of the leaves may belong to another stream, which a capture does not survive
         raise RuntimeError("linear_mxfp4 builds no autograd graph under graph capture: call ops.linear_mxfp4 and "
                            "grad_ops.linear_mxfp4_bwd")
-    if weight.stride(1) != 1 or not x.is_contiguous():
-        x, weight = x.contiguous(), weight.contiguous()
+    x, weight = x.contiguous(), weight.contiguous()
     if x.dim() == 2:
         return _LinearMxfp4Fn.apply(x, weight, bias)
     y = _LinearMxfp4Fn.apply(x.reshape(-1, x.shape[-1]), weight, bias)
@@ -592,7 +593,7 @@ def split_for_muon(named_parameters):
     (embeddings, projections, norms, biases, the logit scale), which stays with `Adam`."""
     matrices, rest = [], []
     for name, p in named_parameters:
-        (matrices if p.dim() == 2 and ".encoder.layers." in name else rest).append(p)
+        (matrices if p.dim() == 2 and "encoder.layers." in name else rest).append(p)
     return matrices, rest
 
 

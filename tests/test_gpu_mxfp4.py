@@ -291,6 +291,26 @@ def test_autograd_shapes_and_partial_gradients():
         assert not training.linear_mxfp4(x, w).requires_grad
 
 
+def test_autograd_of_empty_and_broadcast_operands():
+    for M, N in ((0, 8), (5, 0), (0, 0)):
+        x, w = torch.randn(M, 64, device="cuda", requires_grad=True), torch.randn(N, 64, device="cuda", requires_grad=True)
+        b = torch.randn(N, device="cuda", requires_grad=True)
+        training.linear_mxfp4(x, w, b).float().sum().backward()
+        assert x.grad.shape == (M, 64) and w.grad.shape == (N, 64) and b.grad.shape == (N,)
+        assert not x.grad.any() and not w.grad.any() and not b.grad.any()
+    row, col = torch.randn(1, 64, device="cuda", requires_grad=True), torch.randn(1, 64, device="cuda", requires_grad=True)
+    y = training.linear_mxfp4(row.expand(6, 64), col.expand(3, 64))
+    dy = torch.randn(6, 3, device="cuda").to(BF16)
+    y.backward(dy)
+    dx, dw, _ = G.linear_mxfp4_bwd(dy, ops.quantize_mxfp4(row.detach().expand(6, 64).contiguous()), ops.quantize_mxfp4(col.detach().expand(3, 64).contiguous()), F32)
+    assert torch.allclose(row.grad, dx.sum(0, keepdim=True), rtol=1e-5, atol=1e-5) and torch.allclose(col.grad, dw.sum(0, keepdim=True), rtol=1e-5, atol=1e-5)
+    # strided x, and a transposed result's gradient
+    wide = torch.randn(9, 2 * 64, device="cuda", requires_grad=True)
+    w = torch.randn(16, 64, device="cuda")
+    (training.linear_mxfp4(wide[:, ::2], w).t().float() * 2).sum().backward()
+    assert not wide.grad[:, 1::2].any() and wide.grad[:, ::2].abs().sum() > 0
+
+
 def test_autograd_is_refused_under_capture():
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
     w = torch.randn(8, 64, device="cuda")
