@@ -209,25 +209,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     const int lh0 = lds_off(wm * SM * 16 + r, q), ll0 = lds_off(wm * SM * 16 + r, 4 + q);
     const int rh0 = OP + lds_off(wn * SN * 16 + r, q), rl0 = OP + lds_off(wn * SN * 16 + r, 4 + q);
     f16x8 l[SM], rh[SN], rl[SN];
-    static_assert(SLOTS >= 2 && (SLOTS - 1) * 2 * PIECES < 64, "outstanding fetches within the counter");
-    // Waits until the stage has landed after which `newer` stages were fetched (all of them in whole, or: everything), for all
-    // waves, with this wave's LDS reads done.
+    constexpr int F = 2 * PIECES, F1 = F / 2;
+    static_assert(SLOTS >= 2 && (SLOTS - 1) * F < 64, "outstanding fetches within the counter");
+    // Waits until at most `newer` of this wave's fetches are outstanding (whole), or none, with its LDS reads done; then for all waves.
     auto landed = [&](auto newer, bool whole) {
-        if (whole) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(newer)::value * 2 * PIECES) : "memory");
+        if (whole) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(newer)::value) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // at stage s, stages up to s + SLOTS - 1 have been fetched as far as there are that many
-    auto next_landed = [&](int s) { landed(std::integral_constant<int, SLOTS - 2>{}, s + SLOTS <= g.kc); };
-    auto fetch = [&](int slot) {
+    // stage s + 1: stages up to s + SLOTS - 1 have been fetched as far as there are that many
+    auto next_landed = [&](int s) { landed(std::integral_constant<int, (SLOTS - 2) * F>{}, s + SLOTS <= g.kc); };
+    // A stage's F fetches start when its slot is free, behind the barrier: the first F1 in that stage's last product, the others in the
+    // next stage's first one, so that they are taken (16 cycles each) as evenly as the products allow.
+    auto fetch = [&](int slot, int from, int to) {
 #pragma unroll
-        for (int p = 0; p < 2 * PIECES; p++) fetch_piece(slots + slot, p);
-        lbase += 128;
-        rbase += 128;
+        for (int p = 0; p < F; p++)
+            if (p >= from && p < to) fetch_piece(slots + slot, p);
+        if (to == F) {
+            lbase += 128;
+            rbase += 128;
+        }
     };
-    for (int s = 0; s < min(SLOTS, g.kc); s++) fetch(s * SLOT);
-    landed(std::integral_constant<int, SLOTS - 1>{}, SLOTS <= g.kc);
+    const int full = g.kc >= SLOTS ? SLOTS - 1 : g.kc;
+    for (int s = 0; s < full; s++) fetch(s * SLOT, 0, F);
+    if (g.kc >= SLOTS) fetch((SLOTS - 1) * SLOT, 0, F1);
+    landed(std::integral_constant<int, (SLOTS - 2) * F + F1>{}, g.kc >= SLOTS);
     constexpr int H = SM / 2;
 #pragma unroll
     for (int i = 0; i < H; i++) l[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
@@ -237,8 +244,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     int slot = 0;
     if (SYM && mw + SM * 16 <= nw) {
         for (int s = 0; s < g.kc; s++) {
+            if (s + SLOTS <= g.kc) fetch(slot == 0 ? (SLOTS - 1) * SLOT : slot - SLOT, F1, F);
             next_landed(s);
-            if (s + SLOTS < g.kc) fetch(slot);
+            if (s + SLOTS < g.kc) fetch(slot, 0, F1);
             slot = slot == (SLOTS - 1) * SLOT ? 0 : slot + SLOT;
         }
         __builtin_amdgcn_s_barrier();      // the one before the staging of the results
@@ -249,7 +257,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
         for (int j = 0; j < SN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rr[j], l[i], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto stage = [&](int s, auto fetching) {
+    // early: the rest of stage s + SLOTS - 1 is fetched; late: the start of stage s + SLOTS
+    auto stage = [&](int s, auto early, auto late) {
+        const int last = slot == 0 ? (SLOTS - 1) * SLOT : slot - SLOT;
         const int next = slot == (SLOTS - 1) * SLOT ? 0 : slot + SLOT;
         const unsigned char *cur = lds + slot, *nxt = lds + next;
 #pragma unroll
@@ -257,6 +267,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
             if (i < SM - H) l[H + i] = *(const f16x8 *)(cur + lh0 + (H + i) * 2048);
 #pragma unroll
             for (int j = i * SN / SM; j < (i + 1) * SN / SM; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+            if constexpr (decltype(early)::value) fetch(last, F1 + i * (F - F1) / SM, F1 + (i + 1) * (F - F1) / SM);
             multiply(i, rh);
         }
 #pragma unroll
@@ -267,31 +278,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
 #pragma unroll
         for (int i = 0; i < H; i++) multiply(i, rh);
         next_landed(s);
-        // The fetches go out one by one between the products: in one burst a wave waits 16 cycles for each to be taken, and the
-        // matrix pipe with it.  Behind the last stage the reads return what the slot held before: not used.
-        constexpr int F = 2 * PIECES, G = SM - H;
+        // behind the last stage the reads return what the slot held before: not used
+        constexpr int G = SM - H;
 #pragma unroll
         for (int i = 0; i < G; i++) {           // lo hi; half of the next stage's hi fragments arrive
-            if constexpr (decltype(fetching)::value) {
-#pragma unroll
-                for (int p = i * F / G; p < (i + 1) * F / G; p++) fetch_piece(slots + slot, p);
-            }
+            if constexpr (decltype(late)::value) fetch(slot, i * F1 / G, (i + 1) * F1 / G);
             if (i < H) l[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
 #pragma unroll
             for (int j = i * SN / G; j < (i + 1) * SN / G; j++) rl[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
             multiply(H + i, rh);
-        }
-        if constexpr (decltype(fetching)::value) {
-            lbase += 128;
-            rbase += 128;
         }
 #pragma unroll
         for (int j = 0; j < SN; j++) rh[j] = rl[j];
         slot = next;
     };
     int s = 0;
-    for (; s + SLOTS < g.kc; s++) stage(s, std::true_type{});
-    for (; s < g.kc; s++) stage(s, std::false_type{});
+    for (; s + SLOTS < g.kc; s++) stage(s, std::true_type{}, std::true_type{});
+    if (s + SLOTS == g.kc) stage(s++, std::true_type{}, std::false_type{});
+    for (; s < g.kc; s++) stage(s, std::false_type{}, std::false_type{});
 
     const float alpha = z ? g.alpha[1] : g.alpha[0];
     if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
