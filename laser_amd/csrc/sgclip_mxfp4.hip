@@ -82,31 +82,30 @@ __device__ __forceinline__ void mx_floats(const MxRaw<T> &x, float (&v)[8]) {
 
 // ---------------------------------------------------------------------------
 // Quantisation: a workgroup takes 64 rows x 256 columns, so that the tile's scales are 512 contiguous bytes; four lanes share
-// a block of 32 and find its maximum with two exchanges.  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written
+// a block of 32 and find its maximum with two exchanges.  ROWS = 1, for few rows: eight workgroups share the tile and write single
+// scale bytes (64 x 1024: 2.2 us instead of 4.5).  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written
 // per element; 73856 x 1024 bf16 in 32 us (6.0 TB/s; 46 us with ordinary loads converted at once).
 // ---------------------------------------------------------------------------
-template <typename T, bool VEC>
+template <typename T, bool VEC, int ROWS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, long long ldx, int rows, int cols,
                                                           unsigned char *__restrict__ codes, unsigned char *__restrict__ scales) {
     __shared__ unsigned char sc[512];
     const int tid = threadIdx.x;
     const long long kp = mx_kp(cols);
     const int kt = (int)(kp / MX_K);
-    const int rb = blockIdx.x / kt, kb = blockIdx.x % kt;
+    constexpr int PARTS = 64 / (8 * ROWS);          // workgroups that share 64 rows
+    const int kb = blockIdx.x % kt, rg = blockIdx.x / kt, rb = rg / PARTS, part = rg % PARTS;
     const int c = tid & 31, k = kb * MX_K + c * 8;
-    MxRaw<T> raw[8];
+    unsigned char *tile = scales + ((long long)rb * (kp / 32) + kb * 8) * 64;
+    MxRaw<T> raw[ROWS];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int row = rb * 64 + (tid >> 5) + 8 * i;
+    for (int i = 0; i < ROWS; i++) {
+        const int row = rb * 64 + (part * ROWS + i) * 8 + (tid >> 5);
         raw[i] = mx_load8<T, VEC, true>(x + min(row, rows - 1) * ldx, k, cols);
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int lr = (tid >> 5) + 8 * i, row = rb * 64 + lr;
-        if (row >= rows) {   // scales behind the last row are read with the tile: keep them defined
-            if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = 0;
-            continue;
-        }
+    for (int i = 0; i < ROWS; i++) {
+        const int lr = (part * ROWS + i) * 8 + (tid >> 5), row = rb * 64 + lr;
         float v[8];
         mx_floats(raw[i], v);
         unsigned am = 0;
@@ -114,12 +113,14 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ 
         for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[j]) & 0x7fffffffu);
         am = max(am, (unsigned)__shfl_xor((int)am, 1, 64));
         am = max(am, (unsigned)__shfl_xor((int)am, 2, 64));
-        const unsigned byte = mx_scale_byte(am);
-        *(unsigned *)(codes + row * (kp / 2) + (k >> 1)) = mx_codes8(v, byte);
-        if ((c & 3) == 0) sc[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = (unsigned char)byte;
+        const unsigned byte = row < rows ? mx_scale_byte(am) : 0u;     // behind the last row: read with the tile, so defined
+        if (row < rows) *(unsigned *)(codes + row * (kp / 2) + (k >> 1)) = mx_codes8(v, byte);
+        if ((c & 3) == 0) (ROWS == 8 ? sc : tile)[(c >> 2) * 64 + (lr & 15) * 4 + (lr >> 4)] = (unsigned char)byte;
     }
-    __syncthreads();
-    if (tid < 128) ((unsigned *)(scales + ((long long)rb * (kp / 32) + kb * 8) * 64))[tid] = ((const unsigned *)sc)[tid];
+    if constexpr (ROWS == 8) {
+        __syncthreads();
+        if (tid < 128) ((unsigned *)tile)[tid] = ((const unsigned *)sc)[tid];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -246,8 +247,60 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 __device__ __forceinline__ i32x8 mx_operand(i32x4 v) { return (i32x8){v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
-// Tile of 2 WT x 2 WT, four waves of WT x WT (32 or 64) each; one 256-deep stage in flight behind the one computed, one barrier
-// per stage.
+// A wave's 16 I rows (m = mw ..) x 16 J columns (n = nw ..) where four columns per access are allowed (g.wide).  Straight from the
+// registers: for bf16 two neighbouring 16-lane rows exchange halves, after which a lane holds eight consecutive columns (64 bytes of
+// a row per instruction; through LDS the round trips of a 256 x 256 tile cost 2 us).  bias: that of column nw, in LDS or global memory.
+// STREAM: non-temporal, for results larger than the caches, where ordinary stores wait for the evictions of the previous
+// tile's lines (73856 x 1024 x 4096: 267 us, non-temporal 223).
+template <int EPI, bool STREAM, int I, int J>
+__device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[I][J], const float *bias, int mw, int nw, int lane) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const int r = lane & 15, q = lane >> 4;
+    auto store = [](auto v, auto *p) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+        else *p = v;
+    };
+#pragma unroll
+    for (int p = 0; p < J / 2; p++) {
+        const int n0 = p * 32 + q * 4, n1 = n0 + 16;
+        f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
+        if (g.bias) {
+            if (nw + n0 < g.N) b0 = *(const f32x4 *)(bias + n0);
+            if (nw + n1 < g.N) b1 = *(const f32x4 *)(bias + n1);
+        }
+#pragma unroll
+        for (int i = 0; i < I; i++) {
+            const int m = mw + i * 16 + r;
+            const f32x4 v0 = acc[i][2 * p] + b0, v1 = acc[i][2 * p + 1] + b1;
+            if constexpr (EPI == MX_RESID) {
+                float *o = (float *)g.out + m * g.ldo + nw;
+                const float *res = g.resid + m * g.ldr + nw;
+                if (m < g.M && nw + n0 < g.N) store(*(const f32x4 *)(res + n0) + v0, (f32x4 *)(o + n0));
+                if (m < g.M && nw + n1 < g.N) store(*(const f32x4 *)(res + n1) + v1, (f32x4 *)(o + n1));
+            } else {
+                bf16x4 o0, o1;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    o0[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v0[e]) : v0[e]);
+                    o1[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v1[e]) : v1[e]);
+                }
+                const u32x2 w0 = __builtin_bit_cast(u32x2, o0), w1 = __builtin_bit_cast(u32x2, o1);
+                const u32x2 lo = __builtin_amdgcn_permlane16_swap(w0[0], w1[0], false, false), hi = __builtin_amdgcn_permlane16_swap(w0[1], w1[1], false, false);
+                const int n = nw + p * 32 + (q & 1) * 16 + (q >> 1) * 8;
+                if (m < g.M && n < g.N) {
+                    bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
+                    if (n + 8 <= g.N) store((u32x4){lo[0], hi[0], lo[1], hi[1]}, (u32x4 *)o);
+                    else *(u32x2 *)o = (u32x2){lo[0], hi[0]};
+                }
+            }
+        }
+    }
+}
+
+// Tile of 2 WT x 2 WT, four waves of WT x WT (32 or 64) each; one 256-deep stage in flight behind the one computed, its scales
+// with it in registers, one barrier per stage.  Bound by the latency of a stage's fetch: 9232 x 768 x 768 9.2 us (scales loaded
+// where they are used, results four columns at a time: 12.6), 1540 x 768 x 768 3.9 us.
 template <int EPI, int WT>
 __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
     constexpr int T = 2 * WT, NT = WT / 16, OP = T * 128;
@@ -281,6 +334,15 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
     for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    unsigned na[2], nb[2];
+    auto fetch_scales = [&](int s) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            na[t] = *(const unsigned *)(wsc + ((s * 8 + t * 4 + q) * 16 + r) * 4);
+            nb[t] = *(const unsigned *)(xs + ((s * 8 + t * 4 + q) * 16 + r) * 4);
+        }
+    };
+    fetch_scales(0);
     fetch(0, lds);
     for (int s = 0; s < ns; s++) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -290,10 +352,13 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
         unsigned sa[2], sb[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            sa[t] = *(const unsigned *)(wsc + ((s * 8 + t * 4 + q) * 16 + r) * 4) >> wsh;
-            sb[t] = *(const unsigned *)(xs + ((s * 8 + t * 4 + q) * 16 + r) * 4) >> xsh;
+            sa[t] = na[t] >> wsh;
+            sb[t] = nb[t] >> xsh;
         }
-        if (s + 1 < ns) fetch(s + 1, lds + ((s + 1) & 1) * 2 * OP);
+        if (s + 1 < ns) {
+            fetch_scales(s + 1);
+            fetch(s + 1, lds + ((s + 1) & 1) * 2 * OP);
+        }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             i32x4 fx[NT], fw[NT];
@@ -310,6 +375,10 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
                 });
             });
         }
+    }
+    if (g.wide) {
+        mx_epilogue<EPI, false>(g, acc, g.bias + nrow, mrow, nrow, lane);
+        return;
     }
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -362,51 +431,6 @@ __device__ __forceinline__ void mxp_multiply(f32x4 (&acc)[8][4], const MxFrags &
 template <int EPI>
 constexpr int mxp_stores() {
     return EPI == MX_RESID ? 32 : 16;
-}
-
-// Straight from the registers: for bf16 two neighbouring 16-lane rows exchange halves, after which a lane holds eight consecutive
-// columns (64 bytes of a row per instruction; through LDS the 16 round trips of a tile cost 2 us).  Non-temporal: ordinary
-// stores wait for the evictions of the previous tile's lines (73856 x 1024 x 4096: 267 us, non-temporal 223).
-template <int EPI>
-__device__ __forceinline__ void mxp_epilogue(const MxGemm &g, const f32x4 (&acc)[8][4], const unsigned char *bias, int mw, int nw, int lane) {
-    const int r = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int p = 0; p < 2; p++) {
-        f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
-        if (g.bias) {
-            b0 = *(const f32x4 *)(bias + (p * 32 + q * 4) * 4);
-            b1 = *(const f32x4 *)(bias + (p * 32 + 16 + q * 4) * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int m = mw + i * 16 + r;
-            const f32x4 v0 = acc[i][2 * p] + b0, v1 = acc[i][2 * p + 1] + b1;
-            if constexpr (EPI == MX_RESID) {
-                const int n = nw + p * 32 + q * 4;
-                if (m < g.M && n < g.N)
-                    __builtin_nontemporal_store(*(const f32x4 *)(g.resid + m * g.ldr + n) + v0, (f32x4 *)((float *)g.out + m * g.ldo + n));
-                if (m < g.M && n + 16 < g.N)
-                    __builtin_nontemporal_store(*(const f32x4 *)(g.resid + m * g.ldr + n + 16) + v1, (f32x4 *)((float *)g.out + m * g.ldo + n + 16));
-            } else {
-                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-                typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-                bf16x4 o0, o1;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    o0[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v0[e]) : v0[e]);
-                    o1[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v1[e]) : v1[e]);
-                }
-                const u32x2 w0 = __builtin_bit_cast(u32x2, o0), w1 = __builtin_bit_cast(u32x2, o1);
-                const u32x2 lo = __builtin_amdgcn_permlane16_swap(w0[0], w1[0], false, false), hi = __builtin_amdgcn_permlane16_swap(w0[1], w1[1], false, false);
-                const int n = nw + p * 32 + (q & 1) * 16 + (q >> 1) * 8;
-                if (m < g.M && n < g.N) {
-                    bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
-                    if (n + 8 <= g.N) __builtin_nontemporal_store((u32x4){lo[0], hi[0], lo[1], hi[1]}, (u32x4 *)o);
-                    else *(u32x2 *)o = (u32x2){lo[0], hi[0]};
-                }
-            }
-        }
-    }
 }
 
 template <int EPI>
@@ -500,7 +524,7 @@ __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, i
         }
         int m0, n0;
         origin(t, m0, n0);
-        mxp_epilogue<EPI>(g, acc, lds + MXP_BIAS + bias * 1024 + wn * 256, m0 + wm * 128, n0 + wn * 64, lane);
+        mx_epilogue<EPI, true>(g, acc, (const float *)(lds + MXP_BIAS + bias * 1024 + wn * 256), m0 + wm * 128, n0 + wn * 64, lane);
         bias = (bias + 1) & 3;
         stored = m0 + 256 <= g.M && n0 + 256 <= g.N;
     }
@@ -627,8 +651,15 @@ static int mx_launch_quantize(const T *x, long long ldx, int rows, int cols, uns
     const bool vec = cols % 8 == 0 && ldx * sizeof(T) % 16 == 0 && ((uintptr_t)x & 15) == 0;
     const long long blocks = ((long long)rows + 63) / 64 * (mx_kp(cols) / MX_K);
     if (!mx_grid_ok("sgclip_mxfp4_quantize", blocks, 256)) return SGCLIP_EINVAL;
-    if (vec) mx_quantize_kernel<T, true><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
-    else mx_quantize_kernel<T, false><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+    if (blocks < device_cus()) {
+        const dim3 grid((unsigned)(blocks * 8));
+        if (vec) mx_quantize_kernel<T, true, 1><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+        else mx_quantize_kernel<T, false, 1><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+    } else {
+        const dim3 grid((unsigned)blocks);
+        if (vec) mx_quantize_kernel<T, true, 8><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+        else mx_quantize_kernel<T, false, 8><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
+    }
     return launch_check("sgclip_mxfp4_quantize");
 }
 
