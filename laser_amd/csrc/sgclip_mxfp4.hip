@@ -665,16 +665,21 @@ static int mx_launch_quantize(const T *x, long long ldx, int rows, int cols, uns
 
 template <int EPI>
 static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
+    const long long cus = device_cus();
     const long long huge = (((long long)g.M + 255) / 256) * (((long long)g.N + 255) / 256);
-    if (g.wide && huge >= device_cus() && huge < (1 << 24)) {
+    const long long big = (((long long)g.M + 127) / 128) * (((long long)g.N + 127) / 128);
+    // 256 x 256 tiles where their rounds over the chip cost less: one takes as long as 2.7 of 128 x 128 tiles (K = 1024: 12.8 us for
+    // one or fewer, 23 - 24 for two; 128 x 128 tiles 10.4 us for 440, 13.9 for 584, 20.7 for 1160, 25 - 29 for 1744; K = 4096: 30 and 60;
+    // 23.4, 32.8, 50.9)
+    if (g.wide && (big + cus - 1) / cus * 10 >= (huge + cus - 1) / cus * 27 && huge < (1 << 24)) {
         if (!lds_attr((const void *)mx_pipe_kernel<EPI>, MXP_LDS)) return SGCLIP_ELAUNCH;
-        mx_pipe_kernel<EPI><<<dim3((unsigned)device_cus()), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
+        mx_pipe_kernel<EPI><<<dim3((unsigned)std::min(cus, huge)), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
         return SGCLIP_OK;
     }
-    // 128 x 128 tiles where they fill the chip, 64 x 64 below that
-    const long long big = (((long long)g.M + 127) / 128) * (((long long)g.N + 127) / 128);
+    // 128 x 128 tiles where they fill the chip, 64 x 64 below that (K = 1024: 6.3 against 4.6 us at 80 of the larger, 7.6 both at 224,
+    // 10.4 against 11.4 at 440)
     if (!mx_grid_ok("sgclip_mxfp4_gemm", big, 256)) return SGCLIP_EINVAL;
-    if (big >= device_cus()) {
+    if (big >= cus) {
         if (!lds_attr((const void *)mx_gemm_kernel<EPI, 64>, 4 * 128 * 128)) return SGCLIP_ELAUNCH;
         mx_gemm_kernel<EPI, 64><<<dim3((unsigned)big), 256, 4 * 128 * 128, stream>>>(g);
     } else {

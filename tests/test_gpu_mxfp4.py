@@ -133,6 +133,14 @@ def test_linear_many_tiles(M, N, K):
         assert torch.equal(ops.linear_mxfp4(xq, wq, b, gelu=True), y)
 
 
+@pytest.mark.parametrize("M,N,K", [(2340, 4100, 200), (5000, 5004, 200), (4700, 4612, 512), (10300, 2564, 700), (20600, 1284, 1300),
+                                   (66000, 516, 64), (4616, 1030, 768), (4600, 1028, 1100), (30000, 300, 40)])
+def test_linear_every_kind_of_tile(M, N, K):
+    """256 x 256 tiles in one round over the chip, in two and in four, ragged; 128 x 128 tiles with columns that allow wide accesses
+    and with columns that do not."""
+    test_linear_many_tiles(M, N, K)
+
+
 def test_linear_views_in_place_and_untouched_neighbours():
     M, N, K = 70, 96, 160
     x = _x(2 * M, K + 9, BF16)[::2, 5:5 + K]
