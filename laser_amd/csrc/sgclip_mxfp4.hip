@@ -82,9 +82,10 @@ __device__ __forceinline__ void mx_floats(const MxRaw<T> &x, float (&v)[8]) {
 
 // ---------------------------------------------------------------------------
 // Quantisation: a workgroup takes 64 rows x 256 columns, so that the tile's scales are 512 contiguous bytes; four lanes share
-// a block of 32 and find its maximum with two exchanges.  ROWS = 1, for few rows: eight workgroups share the tile and write single
-// scale bytes (64 x 1024: 2.2 us instead of 4.5).  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written
-// per element; 73856 x 1024 bf16 in 32 us (6.0 TB/s; 46 us with ordinary loads converted at once).
+// a block of 32 and find its maximum with two exchanges.  ROWS = 1, for float inputs and for few rows: eight workgroups share the
+// tile and write single scale bytes (bf16 64 x 1024 2.2 us, ROWS = 8 3.7; 4096 x 1024 3.6, 4.3; 16384 x 1024 10.3, 9.0; float
+// 64 x 1024 2.2, 3.8; 32768 x 4096 104, 128).  Bound by HBM: 2 (bf16) or 4 (f32) bytes read and 17 / 32 written per element;
+// 73856 x 1024 bf16 in 34 us (5.7 TB/s; 46 us with ordinary loads converted at once).
 // ---------------------------------------------------------------------------
 template <typename T, bool VEC, int ROWS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, long long ldx, int rows, int cols,
@@ -650,12 +651,13 @@ template <typename T>
 static int mx_launch_quantize(const T *x, long long ldx, int rows, int cols, unsigned char *codes, unsigned char *scales, hipStream_t stream) {
     const bool vec = cols % 8 == 0 && ldx * sizeof(T) % 16 == 0 && ((uintptr_t)x & 15) == 0;
     const long long blocks = ((long long)rows + 63) / 64 * (mx_kp(cols) / MX_K);
-    if (!mx_grid_ok("sgclip_mxfp4_quantize", blocks, 256)) return SGCLIP_EINVAL;
-    if (blocks < device_cus()) {
+    const bool spread = sizeof(T) == 4 || blocks < 2 * device_cus();
+    if (!mx_grid_ok("sgclip_mxfp4_quantize", spread ? blocks * 8 : blocks, 256)) return SGCLIP_EINVAL;
+    if (spread) {
         const dim3 grid((unsigned)(blocks * 8));
         if (vec) mx_quantize_kernel<T, true, 1><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
         else mx_quantize_kernel<T, false, 1><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
-    } else {
+    } else if constexpr (sizeof(T) == 2) {
         const dim3 grid((unsigned)blocks);
         if (vec) mx_quantize_kernel<T, true, 8><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
         else mx_quantize_kernel<T, false, 8><<<grid, 256, 0, stream>>>(x, ldx, rows, cols, codes, scales);
