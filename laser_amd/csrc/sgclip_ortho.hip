@@ -15,13 +15,20 @@
 // at a third of the fp16 matrix rate.  Powers of two keep the halves inside fp16's range; they are chosen on the host from
 // bounds of the polynomial over the range of singular values.
 //
-// Storage of an operand with K columns ("split rows"): row stride ceil(K / 32) * 128 bytes, per 32 columns 64 bytes of hi and
-// 64 of lo, zeros behind K.  One such piece of a row is a cache line and one stage of the product's loop.
+// A bf16 matrix scaled by a power of two fits one fp16 half, and stays so ("plain") until the first block has been applied to it:
+// its Gram matrix is one product and Q X two (24 of 1024 x 4096: 157 us instead of 360 and 403 instead of 529, and 113 instead of
+// 195 to lay them out; 2.12 ms instead of 2.47 in all).  What the power leaves of 2^e / (|U| + eps), a factor rho in [1, 2) of
+// each matrix, multiplies the products' results.
+//
+// Storage of an operand with K columns: "split rows" with row stride ceil(K / 32) * 128 bytes, per 32 columns 64 bytes of hi and
+// 64 of lo; "plain rows" of fp16 with row stride ceil(K / 64) * 128 bytes; zeros behind K.  A stage of the product's loop is one
+// piece of 128 bytes of each row of split operands, 64 bytes of a plain operand beside it, or 128 of two plain ones.
 #include "tile_common.h"
 
 #include <math.h>
 
 #include <type_traits>
+#include <utility>
 
 namespace sgclip {
 
@@ -33,6 +40,8 @@ constexpr int OR_BATCH = 64;      // matrices per launch: their pointers travel 
 constexpr int OR_PARTS = 64;      // partial sums of a matrix's squared norm
 
 static __host__ __device__ inline int or_chunks(int k) { return (k + 31) / 32; }
+static __host__ __device__ inline int or_split_ld(int k) { return (k + 31) / 32 * 128; }
+static __host__ __device__ inline int or_plain_ld(int k) { return (k + 63) / 64 * 128; }
 
 struct OrPointers {
     void *p[OR_BATCH];
@@ -44,9 +53,10 @@ __device__ __forceinline__ void or_split(float v, f16_t &hi, f16_t &lo) {
 }
 
 // ---------------------------------------------------------------------------
-// The products.  out[i][j] = sum_k L[i][k] R[j][k] on split rows, tile of 2 WT x 2 WT, four waves of WT x WT.
+// The products.  out[i][j] = sum_k L[i][k] R[j][k].
 // ---------------------------------------------------------------------------
 enum { OR_SYM = 0, OR_POLY = 1, OR_BOTH = 2, OR_OUT = 3, OR_UPDATE = 4 };
+enum { OR_SPLIT = 0, OR_PLAIN = 1, OR_PLAIN_R = 2, OR_PLAIN_L = 3 };     // both operands split, both plain, one plain
 
 struct OrGemm {
     const unsigned char *L[2], *R;     // [2]: two products with the same R in one launch (grid z)
@@ -58,8 +68,9 @@ struct OrGemm {
     float ca, cb;                      // OR_POLY: out = alpha (ca I + cb A + A A), the first two in the accumulators from the start
     float decay, rate;                 // OR_UPDATE: p = decay p - rate out
     long long ldo;                     // OR_OUT / OR_UPDATE: row stride in elements
-    int M, N, kc, ldk;                 // rows of L, rows of R, 32-column pieces of both to walk (0: none), bytes of their rows
+    int M, N, kc, ldl, ldr;            // rows of L, rows of R, stages (0: none), bytes of their rows
     int tiles_m, tiles_n, wide;
+    const float *rho;                  // with plain operands: each matrix's factor, once for every plain operand
     OrPointers out;                    // OR_OUT: bf16, OR_UPDATE: f32 parameters
 };
 
@@ -143,17 +154,19 @@ __device__ __forceinline__ void or_symmetrize(f32x4 &v, unsigned char *region, i
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// WM x WN waves of 16 SM rows x 16 SN columns.  SLOTS LDS slots of one 32-column stage each; per stage three products, hi hi, hi lo and
-// lo hi (of L and R).  Fragments roll through one set of registers: those of L arrive a few products before their use and are
-// replaced, hi by lo, row by row; in the middle of the last product every wave holds the rest of the stage, the next stage has
-// landed (the one barrier), and the DMA of stage s + SLOTS starts into the slot just freed.
+// WM x WN waves of 16 SM rows x 16 SN columns.  SLOTS LDS slots of one stage each (32 columns, with OR_PLAIN 64); per stage
+// three products, hi hi, hi lo and lo hi (of L and R), or with plain operands two: hi x and lo x, or the first and the last 32
+// columns.  Fragments roll through one set of registers: those of L arrive a few products before their use and are replaced, hi
+// by lo, row by row; in the middle of the last product every wave holds the rest of the stage, the next stage has landed (the
+// one barrier), and the DMA of stage s + SLOTS starts into the slot just freed.
 //   256 x 256: eight waves, 243 registers, 16.1 results per cycle and CU of 21.3 the matrix pipe could do;
 //   192 x 192: eight waves, three slots; 128 x 128: four waves, two workgroups on a CU; both spend 89 - 100 % of the LDS's cycles;
 //   64 x 64: four waves, four slots, for few tiles, where a stage is shorter than its fetch.
-template <int EPI, int WM, int WN, int SM, int SN, int SLOTS>
+template <int EPI, int FORM, int WM, int WN, int SM, int SN, int SLOTS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
-    constexpr int W = WM * WN, T = WM * SM * 16, OP = T * 128, PIECES = T / 8 / W, SLOT = 2 * OP;
-    static_assert(T == WN * SN * 16 && PIECES * W * 8 == T, "square tiles, whole pieces per wave");
+    constexpr int W = WM * WN, T = WM * SM * 16, LB = FORM == OR_PLAIN_L ? 64 : 128, RB = FORM == OR_PLAIN_R ? 64 : 128;   // bytes of a row's stage
+    constexpr int OP = T * LB, SLOT = OP + T * RB, LP = OP / 1024 / W, RP = T * RB / 1024 / W;
+    static_assert(T == WN * SN * 16 && LP * W * 1024 == OP && RP * W * 1024 == T * RB, "square tiles, whole pieces per wave");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, r = lane & 15, q = lane >> 4;
@@ -174,19 +187,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     ti = __builtin_amdgcn_readfirstlane(ti);
     tj = __builtin_amdgcn_readfirstlane(tj);
     const int m0 = ti * T, n0 = tj * T;
-    const long long ld = (long long)g.ldk, ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
+    const long long ldn = (long long)or_chunks(g.N) * 128, ldm = (long long)or_chunks(g.M) * 128;
 
-    // DMA of a stage: the wave's pieces of 8 rows, wave + W p, rows behind the matrix clamped to its last one
-    const int prow = wave * 8 + (lane >> 3);
-    const unsigned chunk = (unsigned)(((lane & 7) ^ ((prow >> 1) & 7)) * 16), voff = (unsigned)(prow * ld) + chunk;
-    const unsigned step = (unsigned)(8 * W * ld);
-    const unsigned maxl = (unsigned)(min(g.M - 1 - m0, T - 1) * ld) + chunk, maxr = (unsigned)(min(g.N - 1 - n0, T - 1) * ld) + chunk;
-    const unsigned char *lbase = (z ? g.L[1] : g.L[0]) + b * g.sL + m0 * ld, *rbase = g.R + b * g.sR + n0 * ld;
+    // DMA of a stage: pieces of 1024 bytes (8 or 16 rows), the wave's wave + W p, rows behind the matrix clamped to its last one
+    auto piece_row = [&](int bytes) { return bytes == 128 ? wave * 8 + (lane >> 3) : wave * 16 + (lane >> 2); };
+    auto piece_chunk = [&](int bytes, int row) {
+        return (unsigned)((bytes == 128 ? (lane & 7) ^ ((row >> 1) & 7) : (lane & 3) ^ ((row >> 2) & 3)) * 16);
+    };
+    const int lrow = piece_row(LB), rrow = piece_row(RB);
+    const unsigned lchunk = piece_chunk(LB, lrow), rchunk = piece_chunk(RB, rrow);
+    const unsigned loff = (unsigned)(lrow * g.ldl) + lchunk, roff = (unsigned)(rrow * g.ldr) + rchunk;
+    const unsigned lstep = (unsigned)(1024 / LB * W * g.ldl), rstep = (unsigned)(1024 / RB * W * g.ldr);
+    const unsigned maxl = (unsigned)(min(g.M - 1 - m0, T - 1) * g.ldl) + lchunk, maxr = (unsigned)(min(g.N - 1 - n0, T - 1) * g.ldr) + rchunk;
+    const unsigned char *lbase = (z ? g.L[1] : g.L[0]) + b * g.sL + m0 * (long long)g.ldl, *rbase = g.R + b * g.sR + n0 * (long long)g.ldr;
     const unsigned slots = (unsigned)(uintptr_t)LDS_PTR(lds) + wave * 1024;
-    // piece p of the next stage to fetch: the wave's PIECES of L, then of R
+    // piece p of the next stage to fetch: the wave's LP of L, then RP of R
     auto fetch_piece = [&](unsigned slot, int p) {
-        if (p < PIECES) p64_dma16(lbase, voff, p * step, maxl, slot + p * (W * 1024));
-        else p64_dma16(rbase, voff, (p - PIECES) * step, maxr, slot + OP + (p - PIECES) * (W * 1024));
+        if (p < LP) p64_dma16(lbase, loff, p * lstep, maxl, slot + p * (W * 1024));
+        else p64_dma16(rbase, roff, (p - LP) * rstep, maxr, slot + OP + (p - LP) * (W * 1024));
     };
     const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16;
     f32x4 acc[SM][SN];
@@ -205,11 +223,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
                 }
             }
         }
-    // lds_off of a row 16 further is 2048 bytes further, with the same chunk order
-    const int lh0 = lds_off(wm * SM * 16 + r, q), ll0 = lds_off(wm * SM * 16 + r, 4 + q);
-    const int rh0 = OP + lds_off(wn * SN * 16 + r, q), rl0 = OP + lds_off(wn * SN * 16 + r, 4 + q);
+    // a row 16 further has the same chunk order
+    auto at = [](int bytes, int row, int chunk) { return bytes == 128 ? lds_off(row, chunk) : row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4); };
+    const int lh0 = at(LB, wm * SM * 16 + r, q), ll0 = at(128, wm * SM * 16 + r, 4 + q);
+    const int rh0 = OP + at(RB, wn * SN * 16 + r, q), rl0 = OP + at(128, wn * SN * 16 + r, 4 + q);
     f16x8 l[SM], rh[SN], rl[SN];
-    constexpr int F = 2 * PIECES, F1 = F / 2;
+    constexpr int F = LP + RP, F1 = F / 2;
     static_assert(SLOTS >= 2 && (SLOTS - 1) * F < 64, "outstanding fetches within the counter");
     // Waits until at most `newer` of this wave's fetches are outstanding (whole), or none, with its LDS reads done; then for all waves.
     auto landed = [&](auto newer, bool whole) {
@@ -227,8 +246,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
         for (int p = 0; p < F; p++)
             if (p >= from && p < to) fetch_piece(slots + slot, p);
         if (to == F) {
-            lbase += 128;
-            rbase += 128;
+            lbase += LB;
+            rbase += RB;
         }
     };
     const int full = g.kc >= SLOTS ? SLOTS - 1 : g.kc;
@@ -237,9 +256,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     landed(std::integral_constant<int, (SLOTS - 2) * F + F1>{}, g.kc >= SLOTS);
     constexpr int H = SM / 2;
 #pragma unroll
-    for (int i = 0; i < H; i++) l[i] = *(const f16x8 *)(lds + lh0 + i * 2048);
+    for (int i = 0; i < H; i++) l[i] = *(const f16x8 *)(lds + lh0 + i * 16 * LB);
 #pragma unroll
-    for (int j = 0; j < SN; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 2048);
+    for (int j = 0; j < SN; j++) rh[j] = *(const f16x8 *)(lds + rh0 + j * 16 * RB);
     // a diagonal tile's wave above the diagonal only fetches: its block is written from below
     int slot = 0;
     if (SYM && mw + SM * 16 <= nw) {
@@ -262,34 +281,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
         const int last = slot == 0 ? (SLOTS - 1) * SLOT : slot - SLOT;
         const int next = slot == (SLOTS - 1) * SLOT ? 0 : slot + SLOT;
         const unsigned char *cur = lds + slot, *nxt = lds + next;
+        constexpr int G = SM - H;
+        constexpr bool L2 = FORM != OR_PLAIN_L, R2 = FORM != OR_PLAIN_R;     // a second half in the stage
 #pragma unroll
         for (int i = 0; i < SM; i++) {          // hi hi; the rest of L's hi fragments and R's lo fragments arrive
-            if (i < SM - H) l[H + i] = *(const f16x8 *)(cur + lh0 + (H + i) * 2048);
+            if (i < G) l[H + i] = *(const f16x8 *)(cur + lh0 + (H + i) * 16 * LB);
+            if constexpr (R2) {
 #pragma unroll
-            for (int j = i * SN / SM; j < (i + 1) * SN / SM; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+                for (int j = i * SN / SM; j < (i + 1) * SN / SM; j++) rl[j] = *(const f16x8 *)(cur + rl0 + j * 2048);
+            }
             if constexpr (decltype(early)::value) fetch(last, F1 + i * (F - F1) / SM, F1 + (i + 1) * (F - F1) / SM);
             multiply(i, rh);
+            if constexpr (FORM != OR_SPLIT && L2) l[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
         }
+        if constexpr (FORM == OR_SPLIT) {
 #pragma unroll
-        for (int i = 0; i < SM; i++) {          // hi lo; L's lo fragments take the places of the hi ones
-            multiply(i, rl);
-            l[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
+            for (int i = 0; i < SM; i++) {      // hi lo; L's lo fragments take the places of the hi ones
+                multiply(i, rl);
+                l[i] = *(const f16x8 *)(cur + ll0 + i * 2048);
+            }
         }
+        // the last product's R, and where the next stage's arrives
+        constexpr bool LO = FORM == OR_PLAIN || FORM == OR_PLAIN_L;
+        auto &rr = LO ? rl : rh, &rn = LO ? rh : rl;
 #pragma unroll
-        for (int i = 0; i < H; i++) multiply(i, rh);
+        for (int i = 0; i < H; i++) multiply(i, rr);
         next_landed(s);
         // behind the last stage the reads return what the slot held before: not used
-        constexpr int G = SM - H;
 #pragma unroll
         for (int i = 0; i < G; i++) {           // lo hi; half of the next stage's hi fragments arrive
             if constexpr (decltype(late)::value) fetch(slot, i * F1 / G, (i + 1) * F1 / G);
-            if (i < H) l[i] = *(const f16x8 *)(nxt + lh0 + i * 2048);
+            if (i < H) l[i] = *(const f16x8 *)(nxt + lh0 + i * 16 * LB);
 #pragma unroll
-            for (int j = i * SN / G; j < (i + 1) * SN / G; j++) rl[j] = *(const f16x8 *)(nxt + rh0 + j * 2048);
-            multiply(H + i, rh);
+            for (int j = i * SN / G; j < (i + 1) * SN / G; j++) rn[j] = *(const f16x8 *)(nxt + rh0 + j * 16 * RB);
+            multiply(H + i, rr);
         }
+        if constexpr (!LO) {
 #pragma unroll
-        for (int j = 0; j < SN; j++) rh[j] = rl[j];
+            for (int j = 0; j < SN; j++) rh[j] = rl[j];
+        }
         slot = next;
     };
     int s = 0;
@@ -297,7 +327,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     if (s + SLOTS == g.kc) stage(s++, std::true_type{}, std::false_type{});
     for (; s < g.kc; s++) stage(s, std::false_type{}, std::false_type{});
 
-    const float alpha = z ? g.alpha[1] : g.alpha[0];
+    float alpha = z ? g.alpha[1] : g.alpha[0];
+    if constexpr (FORM != OR_SPLIT) alpha *= FORM == OR_PLAIN ? g.rho[b] * g.rho[b] : g.rho[b];
     if constexpr (EPI == OR_OUT || EPI == OR_UPDATE) {
 #pragma unroll
         for (int i = 0; i < SM; i++)
@@ -404,16 +435,16 @@ __global__ __launch_bounds__(256) void or_norm_kernel(OrInput a, double *__restr
     float *buf = (float *)a.buf.p[blockIdx.y];
     double s = 0.0;
     const int step = a.vec ? 4 : 1, per = a.cols / step;
-    const long long total = (long long)a.rows * per;
+    const long long total = (long long)a.rows * per;     // 65536^2 at most: i fits 32 bits
 #pragma unroll 4
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256 * OR_PARTS) {
-        const long long row = i / per;
-        const int col = (int)(i - row * per) * step;
+        long long at = i * step;
+        if (a.ldg != a.cols) at += (unsigned)i / (unsigned)per * (a.ldg - a.cols);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f), m = v;
-        if (a.vec) v = or_load4(g + row * a.ldg + col);
-        else v.x = (float)g[row * a.ldg + col];
+        if (a.vec) v = or_load4(g + at);
+        else v.x = (float)g[at];
         if constexpr (STEP) {
-            float *bp = buf + row * a.cols + col;
+            float *bp = buf + i * step;
             if (a.vec) m = *(const float4 *)bp;
             else m.x = *bp;
             m.x = a.mu * m.x + (1.0f - a.mu) * v.x;
@@ -434,11 +465,13 @@ __global__ __launch_bounds__(256) void or_norm_kernel(OrInput a, double *__restr
     if (threadIdx.x == 0) parts[blockIdx.y * OR_PARTS + blockIdx.x] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
 }
 
-// 64 x 64 tiles: rows [rows][cols] and their transpose [cols][rows], both in split rows, scaled by 2^e / (norm + eps)
+// 64 x 64 tiles: rows [rows][cols] and their transpose [cols][rows].  Split rows scaled by 2^e / (norm + eps); of bf16 matrices plain
+// ones, exact but for what lies 2^-39 below the norm, scaled by the power of two below that, the rest of it in rho.
 template <typename T, bool STEP>
 __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *__restrict__ parts, float scale, float eps,
                                                        unsigned char *__restrict__ rowp, unsigned char *__restrict__ colp,
-                                                       long long srow, long long scol) {
+                                                       long long srow, long long scol, float *__restrict__ rho) {
+    constexpr bool PLAIN = sizeof(T) == 2;
     __shared__ float tile[64][65];
     __shared__ double inv_s;
     const int tid = threadIdx.x, b = blockIdx.y;
@@ -446,7 +479,17 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
         double s = parts[b * OR_PARTS + tid];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (tid == 0) inv_s = (double)scale / (sqrt(s) + (double)eps);
+        if (tid == 0) {
+            const double inv = (double)scale / (sqrt(s) + (double)eps);
+            inv_s = inv;
+            if constexpr (PLAIN) {
+                // the power of two: inv without its fraction; nothing (norm not finite), infinities and NaN stay what they are
+                const double p = __longlong_as_double(__double_as_longlong(inv) & 0x7ff0000000000000LL);
+                const bool usual = p > 0.0 && p <= 1.7976931348623157e308;
+                if (usual) inv_s = p;
+                if (blockIdx.x == 0) rho[b] = usual ? (float)(inv / p) : 1.0f;
+            }
+        }
     }
     __syncthreads();
     const double inv = inv_s;
@@ -478,7 +521,26 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
         }
     }
     __syncthreads();
-    const long long ldr = (long long)or_chunks(a.cols) * 128, ldc = (long long)or_chunks(a.rows) * 128;
+    if constexpr (PLAIN) {
+        const long long ldr = or_plain_ld(a.cols), ldc = or_plain_ld(a.rows);
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const int lr = (tid >> 3) + 32 * p, l8 = (tid & 7) * 8;
+            f16x8 v;
+            if (r0 + lr < a.rows) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = (f16_t)tile[lr][l8 + e];
+                *(f16x8 *)(rowp + b * srow + (r0 + lr) * ldr + (c0 + l8) * 2) = v;
+            }
+            if (c0 + lr < a.cols) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = (f16_t)tile[l8 + e][lr];
+                *(f16x8 *)(colp + b * scol + (c0 + lr) * ldc + (r0 + l8) * 2) = v;
+            }
+        }
+        return;
+    }
+    const long long ldr = or_split_ld(a.cols), ldc = or_split_ld(a.rows);
 #pragma unroll
     for (int p = 0; p < 2; p++) {
         const int lr = (tid >> 3) + 32 * p, l8 = (tid & 7) * 8;
@@ -515,7 +577,7 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
 // ---------------------------------------------------------------------------
 struct OrPlan {
     int m, n, flip;                          // short and long side; flip: the matrix has more rows than columns
-    size_t x, xt, sq, parts, total;          // bytes per matrix: X, X^T, one m x m operand; the norm's parts; all of it
+    size_t x, xt, sq, total;                 // bytes per matrix: X, X^T, one m x m operand; all of it
 };
 
 static OrPlan or_plan(int rows, int cols) {
@@ -523,11 +585,10 @@ static OrPlan or_plan(int rows, int cols) {
     p.flip = rows > cols;
     p.m = p.flip ? cols : rows;
     p.n = p.flip ? rows : cols;
-    p.x = (size_t)p.m * or_chunks(p.n) * 128;
-    p.xt = (size_t)p.n * or_chunks(p.m) * 128;
-    p.sq = (size_t)p.m * or_chunks(p.m) * 128;
-    p.parts = OR_PARTS * sizeof(double);
-    p.total = p.x + 2 * p.xt + 5 * p.sq + p.parts;
+    p.x = (size_t)p.m * or_split_ld(p.n);
+    p.xt = (size_t)p.n * or_split_ld(p.m);
+    p.sq = (size_t)p.m * or_split_ld(p.m);
+    p.total = p.x + 2 * p.xt + 5 * p.sq + (OR_PARTS + 1) * sizeof(double);     // with the norm's parts and rho
     return p;
 }
 
@@ -586,15 +647,15 @@ static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSc
     return or_exponent(top, o.ex[o.blocks]);
 }
 
-template <int EPI, int WM, int WN, int SM, int SN, int SLOTS>
+template <int EPI, int FORM, int WM, int WN, int SM, int SN, int SLOTS>
 static int or_launch_tile(const OrGemm &g, long long blocks, int products, hipStream_t stream) {
-    constexpr int LDS = SLOTS * 2 * (WM * SM * 16) * 128;
-    if (!lds_attr((const void *)or_gemm_kernel<EPI, WM, WN, SM, SN, SLOTS>, LDS)) return SGCLIP_ELAUNCH;
-    or_gemm_kernel<EPI, WM, WN, SM, SN, SLOTS><<<dim3((unsigned)blocks, 1, products), 64 * WM * WN, LDS, stream>>>(g);
+    constexpr int LDS = SLOTS * (WM * SM * 16) * (FORM == OR_PLAIN_L || FORM == OR_PLAIN_R ? 192 : 256);
+    if (!lds_attr((const void *)or_gemm_kernel<EPI, FORM, WM, WN, SM, SN, SLOTS>, LDS)) return SGCLIP_ELAUNCH;
+    or_gemm_kernel<EPI, FORM, WM, WN, SM, SN, SLOTS><<<dim3((unsigned)blocks, 1, products), 64 * WM * WN, LDS, stream>>>(g);
     return launch_check("sgclip_orthogonalize");
 }
 
-template <int EPI>
+template <int EPI, int FORM = OR_SPLIT>
 static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t stream) {
     OrGemm g = gin;
     constexpr bool SYM = EPI == OR_SYM || EPI == OR_POLY;
@@ -612,12 +673,15 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
     // 192 x 192, 2330 for two 128 x 128 tiles that share a CU (16.1, 15.4 and 14.1 results per cycle: the larger the tile, the less LDS
     // traffic per product).  48 of 768 x 768: 192 where X is written (3 rounds), 128 on the triangles; 24 of 1024 x 4096: 256.
     const int cus = device_cus();
-    if (tiles(128) * products < cus) return or_launch_tile<EPI, 2, 2, 2, 2, 4>(g, tiles(64), products, stream);
+    constexpr bool HALF = FORM == OR_PLAIN_L || FORM == OR_PLAIN_R;     // smaller stages: three slots instead of two
+    if (tiles(128) * products < cus) return or_launch_tile<EPI, FORM, 2, 2, 2, 2, 4>(g, tiles(64), products, stream);
     auto cost = [&](int T, int slots, int cycles) { return (tiles(T) * products + slots - 1) / slots * cycles; };
     const long long c128 = cost(128, 2 * cus, 2330), c192 = cost(192, cus, 2400), c256 = cost(256, cus, 4080);
-    if (c256 <= c192 && c256 <= c128) return or_launch_tile<EPI, 2, 4, 8, 4, 2>(g, tiles(256), products, stream);
-    if (c192 < c128) return or_launch_tile<EPI, 2, 4, 6, 3, 3>(g, tiles(192), products, stream);
-    return or_launch_tile<EPI, 2, 2, 4, 4, 2>(g, tiles(128), products, stream);
+    if (c256 <= c128 && (HALF || c256 <= c192)) return or_launch_tile<EPI, FORM, 2, 4, 8, 4, HALF ? 3 : 2>(g, tiles(256), products, stream);
+    if constexpr (!HALF) {     // pieces of a 64-byte operand do not divide a 192 x 192 tile among eight waves
+        if (c192 < c128) return or_launch_tile<EPI, FORM, 2, 4, 6, 3, 3>(g, tiles(192), products, stream);
+    }
+    return or_launch_tile<EPI, FORM, 2, 2, 4, 4, HALF ? 3 : 2>(g, tiles(128), products, stream);
 }
 
 static inline float or_pow2(int e) { return ldexpf(1.0f, e); }
@@ -630,12 +694,14 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
     unsigned char *X = ws, *XT = X + p.x * batch, *XT2 = XT + p.xt * batch, *A = XT2 + p.xt * batch, *M = A + p.sq * batch, *Tm = M + p.sq * batch,
                   *Q = Tm + p.sq * batch, *Q2 = Q + p.sq * batch;
     double *parts = (double *)(Q2 + p.sq * batch);
+    float *rho = (float *)(parts + (size_t)OR_PARTS * batch);
+    bool plain = sizeof(T) == 2;     // X and X^T, until the first block has been applied
     or_norm_kernel<T, STEP><<<dim3(OR_PARTS, batch), 256, 0, stream>>>(in, parts);
     const int tiles = ceil_div(in.rows, 64) * ceil_div(in.cols, 64);
     or_split_kernel<T, STEP><<<dim3(tiles, batch), 256, 0, stream>>>(in, parts, or_pow2(sch.ex[0]), eps, p.flip ? XT : X, p.flip ? X : XT,
-                                                                     p.flip ? p.xt : p.x, p.flip ? p.x : p.xt);
+                                                                     p.flip ? p.xt : p.x, p.flip ? p.x : p.xt, rho);
     int rc = launch_check("sgclip_orthogonalize");
-    const int km = or_chunks(p.m), kn = or_chunks(p.n);
+    const int km = or_chunks(p.m);
     for (int blk = 0, k = 0; blk < sch.blocks && rc == SGCLIP_OK; blk++) {
         int ea = sch.ea0[blk], eq = 0;
         OrGemm g{};
@@ -644,13 +710,14 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
         g.O[0] = A;
         g.sL = g.sR = (long long)p.x;
         g.sO = (long long)p.sq;
-        g.kc = kn;
-        g.ldk = kn * 128;
+        g.ldl = g.ldr = plain ? or_plain_ld(p.n) : or_split_ld(p.n);
+        g.kc = g.ldl / 128;
+        g.rho = rho;
         g.alpha[0] = or_pow2(ea - 2 * sch.ex[blk]);
-        rc = or_launch<OR_SYM>(g, batch, 1, stream);
+        rc = plain ? or_launch<OR_SYM, OR_PLAIN>(g, batch, 1, stream) : or_launch<OR_SYM>(g, batch, 1, stream);
         g.sL = g.sR = g.sA = (long long)p.sq;
         g.kc = km;
-        g.ldk = km * 128;
+        g.ldl = g.ldr = or_split_ld(p.m);
         for (int i = 0; i < sch.len[blk] && rc == SGCLIP_OK; i++, k++) {
             const OrStep &s = sch.s[k];
             const bool last = i + 1 == sch.len[blk];
@@ -702,6 +769,7 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
         g.R = XT;
         g.sL = (long long)p.sq;
         g.sR = (long long)p.xt;
+        g.ldr = plain ? or_plain_ld(p.m) : or_split_ld(p.m);
         g.M = p.m;
         g.N = p.n;
         if (blk + 1 < sch.blocks) {
@@ -710,7 +778,8 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
             g.OT = XT2;
             g.sOT = (long long)p.xt;
             g.alpha[0] = or_pow2(sch.ex[blk + 1] - eq - sch.ex[blk]);
-            rc = or_launch<OR_BOTH>(g, batch, 1, stream);
+            rc = plain ? or_launch<OR_BOTH, OR_PLAIN_R>(g, batch, 1, stream) : or_launch<OR_BOTH>(g, batch, 1, stream);
+            plain = false;
             unsigned char *swap = XT;
             XT = XT2;
             XT2 = swap;
@@ -720,6 +789,7 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
                 g.R = Q;
                 g.sL = (long long)p.xt;
                 g.sR = (long long)p.sq;
+                std::swap(g.ldl, g.ldr);
                 g.M = p.n;
                 g.N = p.m;
             }
@@ -730,7 +800,9 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
             g.rate = rate;
             g.wide = g.N % 4 == 0 && ldo % 4 == 0;
             for (int i = 0; i < batch; i++) g.wide = g.wide && ((uintptr_t)out.p[i] & 15) == 0;
-            rc = STEP ? or_launch<OR_UPDATE>(g, batch, 1, stream) : or_launch<OR_OUT>(g, batch, 1, stream);
+            if constexpr (STEP) rc = or_launch<OR_UPDATE>(g, batch, 1, stream);
+            else if (!plain) rc = or_launch<OR_OUT>(g, batch, 1, stream);
+            else rc = p.flip ? or_launch<OR_OUT, OR_PLAIN_L>(g, batch, 1, stream) : or_launch<OR_OUT, OR_PLAIN_R>(g, batch, 1, stream);
         }
     }
     return rc;

@@ -145,6 +145,51 @@ def test_zero_and_not_finite_matrices_stay_by_themselves():
         assert rel(y[0], iterate(g[0])) <= 3 * tolerance(rows, cols, iterate(g[0])) + UBF
 
 
+def rounded(x, want, tol):
+    """x, rounded to bf16 from something within tol of want, is as far from want as its rounding: rms of as many half steps as
+    elements, equal for both but for four standard deviations of a mean square over them."""
+    return rel(x, want) <= rel(want.to(BF16), want) * (1 + 4 / math.sqrt(want.numel())) + tol
+
+
+@pytest.mark.parametrize("steps", [1, 5, 7])
+@pytest.mark.parametrize("batch,rows,cols", [(2, 100, 120), (2, 120, 100), (70, 65, 130), (40, 200, 330), (9, 900, 400), (3, 1030, 2200), (2, 2200, 1030)])
+def test_bf16_matrices(batch, rows, cols, steps):
+    """bf16 matrices enter the first products unsplit: every tile, both orientations, one block and several."""
+    x = spectrum("strong directions", rows, cols, batch).to(BF16)
+    want = iterate(x, steps)
+    assert rounded(G.orthogonalize(x, steps=steps), want, tolerance(rows, cols, want / math.sqrt(batch)))
+
+
+@pytest.mark.parametrize("rows,cols", [(150, 200), (700, 300)])
+def test_bf16_matrices_of_any_size(rows, cols):
+    g = spectrum("gaussian", rows, cols, 3).to(BF16)
+    g[1] *= 3.0
+    want = iterate(g)
+    tol = tolerance(rows, cols, want / math.sqrt(3))
+    for scale in (1.0, 2.0 ** 100, 2.0 ** -100, 1.7):
+        x = g * scale
+        assert rounded(G.orthogonalize(x, eps=0.0), want if scale != 1.7 else iterate(x), tol)
+    x = g * 2.0 ** -30      # eps counts
+    assert rounded(G.orthogonalize(x), iterate(x), tol)
+    x = (g.double() * torch.exp(-24 * torch.rand(g.shape, device="cuda", dtype=F64))).to(BF16)     # elements of every size down to e^-24
+    assert rounded(G.orthogonalize(x), iterate(x), tolerance(rows, cols, iterate(x) / math.sqrt(3)))
+
+
+def test_bf16_zero_and_not_finite_matrices_stay_by_themselves():
+    for rows, cols in ((70, 50), (300, 400)):
+        g = torch.randn(6, rows, cols, device="cuda").to(BF16)
+        g[1] = 0
+        g[2, 3, 4] = float("nan")
+        g[3, 5, 6] = float("inf")
+        g[5] = 0
+        for eps in (1e-7, 0.0):
+            y = G.orthogonalize(g, eps=eps)
+            assert not y[1].any() if eps else torch.isnan(y[1]).all()
+            assert torch.isnan(y[2]).any() and torch.isnan(y[3]).any()
+            for i in (0, 4):
+                assert rel(y[i], iterate(g[i])) <= 3 * tolerance(rows, cols, iterate(g[i])) + UBF
+
+
 def test_views_outputs_and_neighbours():
     base = torch.randn(5, 90, 140, device="cuda")
     for dtype in (F32, BF16):
