@@ -200,7 +200,7 @@ struct MxGemm {
     void *out;
     long long ldr, ldo, kp;
     int M, N;
-    int wide;    // out, bias, resid allow four columns per access
+    int wide;    // out, bias, resid allow four columns per access; 2: and the rows of out begin on cache lines
 };
 
 // x sigmoid(1.702 x) on the hardware's exp2 and reciprocal (a few 2^-24, far below the bf16 rounding that follows; with an exact
@@ -248,12 +248,23 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 __device__ __forceinline__ i32x8 mx_operand(i32x4 v) { return (i32x8){v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
+// a's lanes of rows 8 .. 15 for b's of rows 0 .. 7 (of 16): afterwards a holds both halves of rows 0 .. 7, b those of rows 8 .. 15
+__device__ __forceinline__ void mx_swap8(unsigned &a, unsigned &b) {
+    const unsigned t = a;
+    a = __builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false);     // row_ror:8 into lanes 8 .. 15
+    b = __builtin_amdgcn_update_dpp(b, t, 0x128, 0xf, 0x3, false);     // and into lanes 0 .. 7
+}
+
 // A wave's 16 I rows (m = mw ..) x 16 J columns (n = nw ..) where four columns per access are allowed (g.wide).  Straight from the
-// registers: for bf16 two neighbouring 16-lane rows exchange halves, after which a lane holds eight consecutive columns (64 bytes of
-// a row per instruction; through LDS the round trips of a 256 x 256 tile cost 2 us).  bias: that of column nw, in LDS or global memory.
+// registers (through LDS the round trips of a 256 x 256 tile cost 2 us): for bf16 two neighbouring 16-lane rows exchange halves, after
+// which a lane holds eight consecutive columns, and an instruction writes 64 bytes of each of 16 rows.  bias: that of column nw, in
+// LDS or global memory.
 // STREAM: non-temporal, for results larger than the caches, where ordinary stores wait for the evictions of the previous
 // tile's lines (73856 x 1024 x 4096: 267 us, non-temporal 223).
-template <int EPI, bool STREAM, int I, int J>
+// LONG: lanes eight apart exchange too, for 128 bytes of each of eight rows: where rows do not begin on cache lines, two accesses to
+// one line cost most (5000 x 200 x 5004 48 us, so 25; on lines they do not, and longer accesses to fewer rows lose: a residual of
+// 73856 x 4096 576 us, so 645).
+template <int EPI, bool STREAM, bool LONG, int I, int J>
 __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[I][J], const float *bias, int mw, int nw, int lane) {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -262,39 +273,82 @@ __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[
         if constexpr (STREAM) __builtin_nontemporal_store(v, p);
         else *p = v;
     };
+    f32x4 b[J];
 #pragma unroll
-    for (int p = 0; p < J / 2; p++) {
-        const int n0 = p * 32 + q * 4, n1 = n0 + 16;
-        f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
-        if (g.bias) {
-            if (nw + n0 < g.N) b0 = *(const f32x4 *)(bias + n0);
-            if (nw + n1 < g.N) b1 = *(const f32x4 *)(bias + n1);
-        }
+    for (int j = 0; j < J; j++) {
+        const int n = j * 16 + q * 4;
+        b[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (g.bias && nw + n < g.N) b[j] = *(const f32x4 *)(bias + n);
+    }
+    if constexpr (EPI == MX_RESID) {
 #pragma unroll
-        for (int i = 0; i < I; i++) {
-            const int m = mw + i * 16 + r;
-            const f32x4 v0 = acc[i][2 * p] + b0, v1 = acc[i][2 * p + 1] + b1;
-            if constexpr (EPI == MX_RESID) {
-                float *o = (float *)g.out + m * g.ldo + nw;
-                const float *res = g.resid + m * g.ldr + nw;
-                if (m < g.M && nw + n0 < g.N) store(*(const f32x4 *)(res + n0) + v0, (f32x4 *)(o + n0));
-                if (m < g.M && nw + n1 < g.N) store(*(const f32x4 *)(res + n1) + v1, (f32x4 *)(o + n1));
-            } else {
-                bf16x4 o0, o1;
+        for (int i = 0; i < I; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    o0[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v0[e]) : v0[e]);
-                    o1[e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(v1[e]) : v1[e]);
+            for (int p = 0; p < J / 2; p++) {
+                unsigned v[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[h][e] = __float_as_uint(acc[i][2 * p + h][e] + b[2 * p + h][e]);
+                if constexpr (LONG) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx_swap8(v[0][e], v[1][e]);
                 }
-                const u32x2 w0 = __builtin_bit_cast(u32x2, o0), w1 = __builtin_bit_cast(u32x2, o1);
-                const u32x2 lo = __builtin_amdgcn_permlane16_swap(w0[0], w1[0], false, false), hi = __builtin_amdgcn_permlane16_swap(w0[1], w1[1], false, false);
-                const int n = nw + p * 32 + (q & 1) * 16 + (q >> 1) * 8;
-                if (m < g.M && n < g.N) {
-                    bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
-                    if (n + 8 <= g.N) store((u32x4){lo[0], hi[0], lo[1], hi[1]}, (u32x4 *)o);
-                    else *(u32x2 *)o = (u32x2){lo[0], hi[0]};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int m = mw + i * 16 + (LONG ? (r & 7) + 8 * h : r), n = nw + p * 32 + (LONG ? r >> 3 : h) * 16 + q * 4;
+                    if (m < g.M && n < g.N) {
+                        const f32x4 res = *(const f32x4 *)(g.resid + m * g.ldr + n);
+                        store(res + __builtin_bit_cast(f32x4, (u32x4){v[h][0], v[h][1], v[h][2], v[h][3]}), (f32x4 *)((float *)g.out + m * g.ldo + n));
+                    }
                 }
             }
+    } else {
+        auto columns = [&](unsigned(&v)[4], int i, int p) {
+            bf16x4 o[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float t = acc[i][2 * p + h][e] + b[2 * p + h][e];
+                    o[h][e] = (bf16_t)(EPI == MX_GELU ? mx_gelu(t) : t);
+                }
+            const u32x2 w0 = __builtin_bit_cast(u32x2, o[0]), w1 = __builtin_bit_cast(u32x2, o[1]);
+            const u32x2 lo = __builtin_amdgcn_permlane16_swap(w0[0], w1[0], false, false), hi = __builtin_amdgcn_permlane16_swap(w0[1], w1[1], false, false);
+            v[0] = lo[0];
+            v[1] = hi[0];
+            v[2] = lo[1];
+            v[3] = hi[1];
+        };
+        auto put = [&](const unsigned(&v)[4], int m, int n) {
+            if (m < g.M && n < g.N) {
+                bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
+                if (n + 8 <= g.N) store((u32x4){v[0], v[1], v[2], v[3]}, (u32x4 *)o);
+                else *(u32x2 *)o = (u32x2){v[0], v[1]};
+            }
+        };
+        const int n = nw + (q & 1) * 16 + (q >> 1) * 8;
+        if constexpr (LONG) {
+            static_assert(J == 4, "64 columns per wave");
+#pragma unroll
+            for (int i = 0; i < I; i++) {
+                unsigned v[2][4];
+                columns(v[0], i, 0);
+                columns(v[1], i, 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx_swap8(v[0][e], v[1][e]);
+                put(v[0], mw + i * 16 + (r & 7), n + (r >> 3) * 32);
+                put(v[1], mw + i * 16 + (r & 7) + 8, n + (r >> 3) * 32);
+            }
+        } else {      // all rows' first halves before the second ones: a line's two stores in a row cost more (228 us, so 217)
+#pragma unroll
+            for (int p = 0; p < J / 2; p++)
+#pragma unroll
+                for (int i = 0; i < I; i++) {
+                    unsigned v[4];
+                    columns(v, i, p);
+                    put(v, mw + i * 16 + r, n + p * 32);
+                }
         }
     }
 }
@@ -378,7 +432,8 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
         }
     }
     if (g.wide) {
-        mx_epilogue<EPI, false>(g, acc, g.bias + nrow, mrow, nrow, lane);
+        if (NT == 2 || g.wide == 2) mx_epilogue<EPI, false, false>(g, acc, g.bias + nrow, mrow, nrow, lane);
+        else mx_epilogue<EPI, false, NT == 4>(g, acc, g.bias + nrow, mrow, nrow, lane);
         return;
     }
 #pragma unroll
@@ -434,7 +489,7 @@ constexpr int mxp_stores() {
     return EPI == MX_RESID ? 32 : 16;
 }
 
-template <int EPI>
+template <int EPI, bool LONG>
 __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, int tiles_n) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -525,7 +580,7 @@ __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, i
         }
         int m0, n0;
         origin(t, m0, n0);
-        mx_epilogue<EPI, true>(g, acc, (const float *)(lds + MXP_BIAS + bias * 1024 + wn * 256), m0 + wm * 128, n0 + wn * 64, lane);
+        mx_epilogue<EPI, true, LONG>(g, acc, (const float *)(lds + MXP_BIAS + bias * 1024 + wn * 256), m0 + wm * 128, n0 + wn * 64, lane);
         bias = (bias + 1) & 3;
         stored = m0 + 256 <= g.M && n0 + 256 <= g.N;
     }
@@ -674,8 +729,9 @@ static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
     // one or fewer, 23 - 24 for two; 128 x 128 tiles 10.4 us for 440, 13.9 for 584, 20.7 for 1160, 25 - 29 for 1744; K = 4096: 30 and 60;
     // 23.4, 32.8, 50.9)
     if (g.wide && (big + cus - 1) / cus * 10 >= (huge + cus - 1) / cus * 27 && huge < (1 << 24)) {
-        if (!lds_attr((const void *)mx_pipe_kernel<EPI>, MXP_LDS)) return SGCLIP_ELAUNCH;
-        mx_pipe_kernel<EPI><<<dim3((unsigned)std::min(cus, huge)), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
+        const auto kernel = g.wide == 2 ? mx_pipe_kernel<EPI, false> : mx_pipe_kernel<EPI, true>;
+        if (!lds_attr((const void *)kernel, MXP_LDS)) return SGCLIP_ELAUNCH;
+        kernel<<<dim3((unsigned)std::min(cus, huge)), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
         return SGCLIP_OK;
     }
     // 128 x 128 tiles where they fill the chip, 64 x 64 below that (K = 1024: 6.3 against 4.6 us at 80 of the larger, 7.6 both at 224,
@@ -718,6 +774,7 @@ static int mx_epilogue(const char *who, MxGemm &g, int epilogue, const float *bi
     g.ldo = ldo;
     g.wide = g.N % 4 == 0 && ldo % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)bias & 15) == 0 &&
              (epi != MX_RESID || (ldaux % 4 == 0 && ((uintptr_t)aux & 15) == 0));
+    if (g.wide && ldo * (epi == MX_RESID ? 4 : 2) % 128 == 0 && ((uintptr_t)out & 127) == 0) g.wide = 2;
     return SGCLIP_OK;
 }
 
