@@ -55,17 +55,27 @@ struct MxRaw {
     T v[8] __attribute__((aligned(16)));
 };
 
-// Eight elements from column k of a row (zeros behind cols).  VEC: 16-byte loads, whole groups of eight only.  STREAM: the
-// elements are not needed again (non-temporal).
+// 16 bytes at any address: global memory takes accesses of four dwords without alignment
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// Eight elements from column k of a row (zeros behind cols).  VEC: aligned rows of whole groups of eight.  STREAM: the elements are
+// not needed again (non-temporal).
 template <typename T, bool VEC, bool STREAM = false>
 __device__ __forceinline__ MxRaw<T> mx_load8(const T *__restrict__ row, int k, int cols) {
     MxRaw<T> x;
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     if constexpr (VEC) {
-        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int j = 0; j < (int)sizeof(T) / 2; j++) {
             const u32x4 *p = (const u32x4 *)(row + k) + j;
             ((u32x4 *)x.v)[j] = k < cols ? (STREAM ? __builtin_nontemporal_load(p) : *p) : (u32x4){0, 0, 0, 0};
+        }
+    } else if (k + 8 <= cols) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) {
+            const u32x4_any *p = (const u32x4_any *)(row + k) + j;
+            ((u32x4 *)x.v)[j] = STREAM ? __builtin_nontemporal_load(p) : *p;
         }
     } else {
 #pragma unroll
@@ -141,7 +151,7 @@ __device__ __forceinline__ float mx_row_scale(const unsigned char *scales, long 
 }
 
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                                            int rows, int cols, bf16_t *__restrict__ out, long long ldo, int vec) {
+                                                            int rows, int cols, bf16_t *__restrict__ out, long long ldo) {
     const long long kp = mx_kp(cols);
     const int per = (cols + 7) / 8;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -151,11 +161,11 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char 
     float v[8];
     mx_values8(*(const unsigned *)(codes + row * (kp / 2) + (k >> 1)), mx_row_scale(scales, kp, row, k >> 5), v);
     bf16_t *o = out + row * ldo + k;
-    if (vec) {
+    if (k + 8 <= cols) {
         bf16x8 b;
 #pragma unroll
         for (int j = 0; j < 8; j++) b[j] = (bf16_t)v[j];
-        *(bf16x8 *)o = b;
+        *(u32x4_any *)o = __builtin_bit_cast(u32x4_any, b);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -200,7 +210,7 @@ struct MxGemm {
     void *out;
     long long ldr, ldo, kp;
     int M, N;
-    int wide;    // out, bias, resid allow four columns per access; 2: and the rows of out begin on cache lines
+    int wide;    // out, bias, resid allow four columns per aligned access; 2: and the rows of out begin on cache lines
 };
 
 // x sigmoid(1.702 x) on the hardware's exp2 and reciprocal (a few 2^-24, far below the bf16 rounding that follows; with an exact
@@ -255,30 +265,38 @@ __device__ __forceinline__ void mx_swap8(unsigned &a, unsigned &b) {
     b = __builtin_amdgcn_update_dpp(b, t, 0x128, 0xf, 0x3, false);     // and into lanes 0 .. 7
 }
 
-// A wave's 16 I rows (m = mw ..) x 16 J columns (n = nw ..) where four columns per access are allowed (g.wide).  Straight from the
+// A wave's 16 I rows (m = mw ..) x 16 J columns (n = nw ..).  Straight from the
 // registers (through LDS the round trips of a 256 x 256 tile cost 2 us): for bf16 two neighbouring 16-lane rows exchange halves, after
 // which a lane holds eight consecutive columns, and an instruction writes 64 bytes of each of 16 rows.  bias: that of column nw, in
-// LDS or global memory.
+// LDS (STREAM: a whole tile's) or global memory.
 // STREAM: non-temporal, for results larger than the caches, where ordinary stores wait for the evictions of the previous
 // tile's lines (73856 x 1024 x 4096: 267 us, non-temporal 223).
 // LONG: lanes eight apart exchange too, for 128 bytes of each of eight rows: where rows do not begin on cache lines, two accesses to
 // one line cost most (5000 x 200 x 5004 48 us, so 25; on lines they do not, and longer accesses to fewer rows lose: a residual of
 // 73856 x 4096 576 us, so 645).
-template <int EPI, bool STREAM, bool LONG, int I, int J>
+// ANY: out, bias and residual at any element, any number of columns (without: g.wide).
+template <int EPI, bool STREAM, bool LONG, bool ANY, int I, int J>
 __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[I][J], const float *bias, int mw, int nw, int lane) {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     const int r = lane & 15, q = lane >> 4;
-    auto store = [](auto v, auto *p) {
-        if constexpr (STREAM) __builtin_nontemporal_store(v, p);
-        else *p = v;
+    auto store = [](u32x4 v, void *at) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, (u32x4_any *)at);
+        else *(u32x4_any *)at = v;
     };
     f32x4 b[J];
 #pragma unroll
     for (int j = 0; j < J; j++) {
         const int n = j * 16 + q * 4;
         b[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (g.bias && nw + n < g.N) b[j] = *(const f32x4 *)(bias + n);
+        if (!g.bias) continue;
+        if constexpr (STREAM) b[j] = *(const f32x4 *)(bias + n);
+        else if (nw + n + (ANY ? 4 : 1) <= g.N) b[j] = *(const f32x4_any *)(bias + n);
+        else if constexpr (ANY) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (nw + n + e < g.N) b[j][e] = bias[n + e];
+        }
     }
     if constexpr (EPI == MX_RESID) {
 #pragma unroll
@@ -297,9 +315,16 @@ __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int m = mw + i * 16 + (LONG ? (r & 7) + 8 * h : r), n = nw + p * 32 + (LONG ? r >> 3 : h) * 16 + q * 4;
-                    if (m < g.M && n < g.N) {
-                        const f32x4 res = *(const f32x4 *)(g.resid + m * g.ldr + n);
-                        store(res + __builtin_bit_cast(f32x4, (u32x4){v[h][0], v[h][1], v[h][2], v[h][3]}), (f32x4 *)((float *)g.out + m * g.ldo + n));
+                    if (m >= g.M) continue;
+                    const float *res = g.resid + m * g.ldr + n;
+                    float *o = (float *)g.out + m * g.ldo + n;
+                    if (n + (ANY ? 4 : 1) <= g.N) {
+                        const f32x4 sum = *(const f32x4_any *)res + __builtin_bit_cast(f32x4, (u32x4){v[h][0], v[h][1], v[h][2], v[h][3]});
+                        store(__builtin_bit_cast(u32x4, sum), o);
+                    } else if constexpr (ANY) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < g.N) o[e] = res[e] + __uint_as_float(v[h][e]);
                     }
                 }
             }
@@ -321,10 +346,14 @@ __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[
             v[3] = hi[1];
         };
         auto put = [&](const unsigned(&v)[4], int m, int n) {
-            if (m < g.M && n < g.N) {
-                bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
-                if (n + 8 <= g.N) store((u32x4){v[0], v[1], v[2], v[3]}, (u32x4 *)o);
-                else *(u32x2 *)o = (u32x2){v[0], v[1]};
+            if (m >= g.M || n >= g.N) return;
+            bf16_t *o = (bf16_t *)g.out + m * g.ldo + n;
+            if (n + 8 <= g.N) store((u32x4){v[0], v[1], v[2], v[3]}, o);
+            else if constexpr (!ANY) *(u32x2 *)o = (u32x2){v[0], v[1]};
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (n + e < g.N) ((unsigned short *)o)[e] = (unsigned short)(v[e >> 1] >> (e & 1) * 16);
             }
         };
         const int n = nw + (q & 1) * 16 + (q >> 1) * 8;
@@ -431,15 +460,8 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
             });
         }
     }
-    if (g.wide) {
-        if (NT == 2 || g.wide == 2) mx_epilogue<EPI, false, false>(g, acc, g.bias + nrow, mrow, nrow, lane);
-        else mx_epilogue<EPI, false, NT == 4>(g, acc, g.bias + nrow, mrow, nrow, lane);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) mx_store4<EPI>(g, acc[i][j], mrow + i * 16 + r, nrow + j * 16 + q * 4);
+    if (g.wide == 2) mx_epilogue<EPI, false, false, false>(g, acc, g.bias + nrow, mrow, nrow, lane);
+    else mx_epilogue<EPI, false, NT == 4, true>(g, acc, g.bias + nrow, mrow, nrow, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -481,6 +503,11 @@ __device__ __forceinline__ void mxp_multiply(f32x4 (&acc)[8][4], const MxFrags &
         __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
         __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
     }
+}
+
+// four bytes a lane (any alignment and number of columns) to 256 consecutive bytes of LDS
+__device__ __forceinline__ void mxp_dma4(const unsigned char *base, int off, unsigned lds_addr) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 1\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 
 // vector memory stores of a wave for a whole tile, all younger than its last fetch
@@ -531,8 +558,13 @@ __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, i
             p64_dma16(wb, voff, p * step, maxw, slot + MXP_OP + (wave + 8 * p) * 1024);
         }
         if (wave < 4) p64_dma16(sb, sc_voff, 0, maxs, slot + 2 * MXP_OP + wave * 1024);
-        else if (wave == 4 && fs == 0 && g.bias)
-            p64_dma16((const unsigned char *)(g.bias + fn0), lane * 16, 0, (unsigned)(min(g.N - fn0, 256) * 4 - 16), lds0 + MXP_BIAS + fbias * 1024);
+        else if (wave == 4 && fs == 0 && g.bias) {
+            if constexpr (LONG) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    mxp_dma4((const unsigned char *)(g.bias + fn0), min(p * 64 + lane, g.N - 1 - fn0) * 4, lds0 + MXP_BIAS + fbias * 1024 + p * 256);
+            } else p64_dma16((const unsigned char *)(g.bias + fn0), lane * 16, 0, (unsigned)(min(g.N - fn0, 256) * 4 - 16), lds0 + MXP_BIAS + fbias * 1024);
+        }
         xb += 128;
         wb += 128;
         sb += 512;
@@ -580,7 +612,7 @@ __global__ __launch_bounds__(512, 2) void mx_pipe_kernel(MxGemm g, int ntiles, i
         }
         int m0, n0;
         origin(t, m0, n0);
-        mx_epilogue<EPI, true, LONG>(g, acc, (const float *)(lds + MXP_BIAS + bias * 1024 + wn * 256), m0 + wm * 128, n0 + wn * 64, lane);
+        mx_epilogue<EPI, true, LONG, LONG>(g, acc, (const float *)(lds + MXP_BIAS + bias * 1024 + wn * 256), m0 + wm * 128, n0 + wn * 64, lane);
         bias = (bias + 1) & 3;
         stored = m0 + 256 <= g.M && n0 + 256 <= g.N;
     }
@@ -728,7 +760,7 @@ static int mx_launch_gemm(const MxGemm &g, hipStream_t stream) {
     // 256 x 256 tiles where their rounds over the chip cost less: one takes as long as 2.7 of 128 x 128 tiles (K = 1024: 12.8 us for
     // one or fewer, 23 - 24 for two; 128 x 128 tiles 10.4 us for 440, 13.9 for 584, 20.7 for 1160, 25 - 29 for 1744; K = 4096: 30 and 60;
     // 23.4, 32.8, 50.9)
-    if (g.wide && (big + cus - 1) / cus * 10 >= (huge + cus - 1) / cus * 27 && huge < (1 << 24)) {
+    if ((big + cus - 1) / cus * 10 >= (huge + cus - 1) / cus * 27 && huge < (1 << 24)) {
         const auto kernel = g.wide == 2 ? mx_pipe_kernel<EPI, false> : mx_pipe_kernel<EPI, true>;
         if (!lds_attr((const void *)kernel, MXP_LDS)) return SGCLIP_ELAUNCH;
         kernel<<<dim3((unsigned)std::min(cus, huge)), 512, MXP_LDS, stream>>>(g, (int)huge, (g.N + 255) / 256);
@@ -818,10 +850,9 @@ int sgclip_mxfp4_dequantize(const void *codes_dev, const void *scales_dev, int r
         if (!mx_grid_ok("sgclip_mxfp4_dequantize", tiles, 256)) return SGCLIP_EINVAL;
         mx_dequantize_t_kernel<<<dim3((unsigned)tiles), 256, 0, (hipStream_t)stream>>>(c, s, rows, cols, (bf16_t *)out_dev, ldo);
     } else {
-        const int vec = cols % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)out_dev & 15) == 0;
         const long long n = (long long)rows * ((cols + 7) / 8);
         if (!mx_grid_ok("sgclip_mxfp4_dequantize", (n + 255) / 256, 256)) return SGCLIP_EINVAL;
-        mx_dequantize_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, (hipStream_t)stream>>>(c, s, rows, cols, (bf16_t *)out_dev, ldo, vec);
+        mx_dequantize_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, (hipStream_t)stream>>>(c, s, rows, cols, (bf16_t *)out_dev, ldo);
     }
     return launch_check("sgclip_mxfp4_dequantize");
 }

@@ -141,6 +141,37 @@ def test_linear_every_kind_of_tile(M, N, K):
     test_linear_many_tiles(M, N, K)
 
 
+@pytest.mark.parametrize("M,N,K", [(2340, 4099, 200), (5000, 5001, 200), (4700, 4614, 131), (20600, 1283, 1301), (66000, 517, 64), (4616, 1031, 767),
+                                   (30000, 301, 40), (300, 131, 77), (90, 33, 1000), (20, 7, 31)])
+def test_linear_of_any_alignment(M, N, K):
+    """Odd row strides and column counts, operands that begin anywhere: every kernel, nothing written beside the result."""
+    x = _x(M, K + 1, BF16)[:, 1:]
+    w = 0.02 * torch.randn(N, K, device="cuda")
+    b = torch.randn(N + 1, device="cuda")[1:]
+    xv, wv = values(x), values(w)
+    xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    assert torch.equal(ops.dequantize_mxfp4(xq).double(), xv)
+    s, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    store = torch.full((M + 2, N + 3), 7.0, device="cuda")
+    out = store[1:-1, 1:1 + N]
+    r = torch.randn(M, N, device="cuda")
+    out.copy_(r)
+    for q in (x, xq):
+        out.copy_(r)
+        ops.linear_mxfp4(q, wq, b, residual=out, out=out)
+        _check(out, r.double() + s + b.double(), size + b.double().abs() + r.double().abs(), K, 2)
+    u = s + b.double()
+    g = u * torch.sigmoid(1.702 * u)
+    err = 1.1 * (K + 1) * U32 * (size + b.double().abs()) + 2.0 ** -20 * g.abs()
+    half = torch.full((M + 2, N + 3), 7.0, dtype=BF16, device="cuda")
+    outh = half[1:-1, 1:1 + N]
+    _check(ops.linear_mxfp4(xq, wq, b, gelu=True, out=outh), g, 0 * size, 0, 0, err + UBF * (g.abs() + err))
+    _check(ops.linear_mxfp4(x, wq, out=outh), s, size, K, 0, UBF * (s.abs() + K * U32 * size))
+    for t in (store, half):
+        t[1:-1, 1:1 + N] = 7.0
+        assert (t == 7.0).all()
+
+
 def test_linear_views_in_place_and_untouched_neighbours():
     M, N, K = 70, 96, 160
     x = _x(2 * M, K + 9, BF16)[::2, 5:5 + K]
