@@ -284,19 +284,28 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
         return (torch.zeros((M, K), dtype=dx_dtype, device=dev) if need_dx else None,
                 torch.zeros((N, K), dtype=F32, device=dev) if need_dw else None, db)
     dyb = cast_bf16(dy) if dy.dtype == F32 else dy
-    dx = None
+    dx = dw = None
+    Np, Kp = pad64(N), (K + 7) // 8 * 8
+    dyp = dyb
+    if (need_dx and N != Np) or (need_dw and N % 8):
+        dyp = torch.empty((M, Np), dtype=BF16, device=dev)
+        dyp[:, :N] = dyb
+        dyp[:, N:] = 0
     if need_dx:
         w_t = dequantize_mxfp4(wq, transpose=True)       # [K, N rounded up to 64], zeros behind N
-        dyp = dyb
-        if w_t.shape[1] != N:
-            dyp = torch.zeros((M, w_t.shape[1]), dtype=BF16, device=dev)
-            dyp[:, :N] = dyb
         dx = torch.empty((M, K), dtype=dx_dtype, device=dev)
         if dx_dtype == F32:
             gemm_bf16(dyp, w_t, dx, _lib.EPI_F32)
         else:
             gemm_bf16(dyp, w_t, dx, _lib.EPI_BIAS_BF16, bias=torch.zeros(K, dtype=F32, device=dev))
-    dw = linear_wgrad(dyb, dequantize_mxfp4(xq)) if need_dw else None
+    if need_dw:
+        # in whole groups of eight columns, as the product takes them from memory: the codes behind the last column are zeros, and
+        # what they and dy's padding give is dropped
+        x = dequantize_mxfp4(Mxfp4(xq.data, M, Kp))
+        if N % 8 == 0 and K == Kp:
+            dw = linear_wgrad(dyb, x)
+        else:
+            dw = linear_wgrad(dyb if N % 8 == 0 else dyp[:, :(N + 7) // 8 * 8], x)[:N, :K].contiguous()
     return dx, dw, db
 
 
