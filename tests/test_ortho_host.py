@@ -29,8 +29,8 @@ def test_workspace_sizes(lib):
     assert need(0, 8, 8) == 0 and need(1, 0, 8) == 0 and need(1, 8, -1) == 0
     assert need(1, 100, 300) == need(1, 300, 100) > 0
     assert need(64, 128, 128) == 64 * need(1, 128, 128) == need(1000, 128, 128)     # larger batches run in groups
-    # operands of 4 bytes an element, padded to 32 columns: X, two X^T, five squares, 64 partial sums
-    assert need(1, 33, 65) == 33 * 3 * 128 + 2 * 65 * 2 * 128 + 5 * 33 * 2 * 128 + 64 * 8
+    # operands of 4 bytes an element, padded to 32 columns: X, two X^T, five squares, 64 partial sums and a factor
+    assert need(1, 33, 65) == 33 * 3 * 128 + 2 * 65 * 2 * 128 + 5 * 33 * 2 * 128 + 65 * 8
 
 
 def test_entry_point_refusals(lib):
