@@ -127,6 +127,9 @@ SIGNATURES = {
     "sgclip_mxfp4_linear_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "sgclip_mxfp4_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                       C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "sgclip_mxfp4_linear_bwd_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "sgclip_mxfp4_linear_bwd": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                          C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "sgclip_column_sums_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "sgclip_column_sums": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "sgclip_orthogonalize_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),

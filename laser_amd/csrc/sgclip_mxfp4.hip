@@ -663,22 +663,22 @@ __global__ __launch_bounds__(1024) void mx_few_rows_kernel(const T *__restrict__
 
 // ---------------------------------------------------------------------------
 // Column sums without atomics (bias gradients): every workgroup sums a strip of rows of 512 columns (a lane eight of them, its
-// four waves every fourth row), a second launch adds the strips in a fixed order.  Bound by HBM: 36928 x 4096 bf16 in 51 us
-// (5.9 TB/s), the second launch 4 us.
+// waves every WAVES-th row), a second launch adds the strips in a fixed order; few rows are one strip of 16 waves, and no second
+// launch.  Bound by HBM: 36928 x 4096 bf16 in 51 us (5.9 TB/s), the second launch 4 us.
 // ---------------------------------------------------------------------------
-constexpr int CS_COLS = 512, CS_STRIPS = 256, CS_ROWS = 32;
+constexpr int CS_COLS = 512, CS_STRIPS = 256, CS_ROWS = 32, CS_FEW = 512;
 
-static inline int cs_strips(int M) { return std::max(1, std::min(CS_STRIPS, (M + CS_ROWS - 1) / CS_ROWS)); }
+static inline int cs_strips(int M) { return M <= CS_FEW ? 1 : std::min(CS_STRIPS, (M + CS_ROWS - 1) / CS_ROWS); }
 
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void mx_colsum_strip_kernel(const T *__restrict__ in, long long ld, int M, int N, float *__restrict__ parts) {
-    __shared__ float sums[4][CS_COLS];
+template <typename T, bool VEC, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mx_colsum_strip_kernel(const T *__restrict__ in, long long ld, int M, int N, float *__restrict__ parts) {
+    __shared__ float sums[WAVES][CS_COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * CS_COLS + lane * 8;
     const long long per = ((long long)M + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per, hi = min(lo + per, (long long)M);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < N) {
 #pragma unroll 4
-        for (long long m = lo + wave; m < hi; m += 4) {
+        for (long long m = lo + wave; m < hi; m += WAVES) {
             float v[8];
             mx_floats(mx_load8<T, VEC>(in + m * ld, n, N), v);
 #pragma unroll
@@ -688,9 +688,13 @@ __global__ __launch_bounds__(256) void mx_colsum_strip_kernel(const T *__restric
 #pragma unroll
     for (int j = 0; j < 8; j++) sums[wave][lane * 8 + j] = s[j];
     __syncthreads();
-    for (int c = threadIdx.x; c < CS_COLS; c += 256)
-        if (blockIdx.x * CS_COLS + c < N)
-            parts[(long long)blockIdx.y * N + blockIdx.x * CS_COLS + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    for (int c = threadIdx.x; c < CS_COLS; c += 64 * WAVES)
+        if (blockIdx.x * CS_COLS + c < N) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w += 4) t += (sums[w][c] + sums[w + 1][c]) + (sums[w + 2][c] + sums[w + 3][c]);
+            parts[(long long)blockIdx.y * N + blockIdx.x * CS_COLS + c] = t;
+        }
 }
 
 __global__ __launch_bounds__(256) void mx_colsum_join_kernel(const float *__restrict__ parts, int strips, int N, float *__restrict__ out) {
@@ -704,6 +708,42 @@ __global__ __launch_bounds__(256) void mx_colsum_join_kernel(const float *__rest
     sums[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && n < N) out[n] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+}
+
+// ---------------------------------------------------------------------------
+// The layer's gradients run on the bf16 products; these lay their operands out.
+// ---------------------------------------------------------------------------
+// [M, N] to bf16 [M, ldo] with zeros behind N; ldo a multiple of 8
+template <typename T>
+__global__ __launch_bounds__(256) void mx_pad_kernel(const T *__restrict__ in, long long ld, int M, int N, bf16_t *__restrict__ out, int ldo) {
+    const int per = ldo / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)M * per) return;
+    const long long row = i / per;
+    const int k = (int)(i - row * per) * 8;
+    float v[8];
+    mx_floats(mx_load8<T, false>(in + row * ld, k, N), v);
+    bf16x8 b;
+#pragma unroll
+    for (int j = 0; j < 8; j++) b[j] = (bf16_t)v[j];
+    *(bf16x8 *)(out + i * 8) = b;
+}
+
+// zeros: where the weight gradient is summed, and the bias that the data gradient's product asks for
+template <typename T>
+__global__ __launch_bounds__(256) void mx_zero_kernel(T *__restrict__ a, long long na, T *__restrict__ b, long long nb) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < na + nb; i += (long long)gridDim.x * 256) {
+        if (i < na) a[i] = (T)0.f;
+        else b[i - na] = (T)0.f;
+    }
+}
+
+__global__ __launch_bounds__(256) void mx_crop_kernel(const float *__restrict__ in, int ldi, int rows, int cols, float *__restrict__ out) {
+    const long long n = (long long)rows * cols;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long row = i / cols;
+        out[i] = in[row * ldi + (i - row * cols)];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -785,6 +825,58 @@ static void mx_launch_few(const T *x, long long ldx, int K, const MxGemm &g, hip
     const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * std::min(16, (K + 127) / 128));
     if (vec) mx_few_rows_kernel<T, true, EPI><<<grid, block, 0, stream>>>(x, ldx, K, g);
     else mx_few_rows_kernel<T, false, EPI><<<grid, block, 0, stream>>>(x, ldx, K, g);
+}
+
+template <typename T>
+static void mx_launch_colsum(const T *in, long long ld, int M, int N, int strips, float *parts, float *out, hipStream_t st) {
+    const bool vec = N % 8 == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t)in & 15) == 0;
+    const dim3 grid((unsigned)ceil_div(N, CS_COLS), (unsigned)strips);
+    if (strips == 1) {
+        if (vec) mx_colsum_strip_kernel<T, true, 16><<<grid, 1024, 0, st>>>(in, ld, M, N, out);
+        else mx_colsum_strip_kernel<T, false, 16><<<grid, 1024, 0, st>>>(in, ld, M, N, out);
+        return;
+    }
+    if (vec) mx_colsum_strip_kernel<T, true, 4><<<grid, 256, 0, st>>>(in, ld, M, N, parts);
+    else mx_colsum_strip_kernel<T, false, 4><<<grid, 256, 0, st>>>(in, ld, M, N, parts);
+    mx_colsum_join_kernel<<<dim3((unsigned)((N + 63) / 64)), 256, 0, st>>>(parts, strips, N, out);
+}
+
+static inline unsigned mx_grid(long long n) { return (unsigned)std::min((n + 255) / 256, 4096LL); }     // for loops over the grid
+
+template <typename T>
+static void mx_zero(T *a, long long na, T *b, long long nb, hipStream_t st) {
+    if (na + nb > 0) mx_zero_kernel<<<dim3(mx_grid(na + nb)), 256, 0, st>>>(a, na, b, nb);
+}
+
+// workspace of the layer's gradients: zeros f32 [K]; dy bf16 [M][n64], if it has to be laid out; w^T bf16 [K][n64]; x bf16 [M][k8];
+// dw f32 [n8][k8], if it has to be cropped; column sums
+struct MxBwdPlan {
+    int n8, n64, k8;
+    bool pad, crop;
+    size_t zeros, dy, wt, x, dw, parts, total;
+};
+
+static MxBwdPlan mx_bwd_plan(const void *dy, int dtype, long long lddy, int M, int N, int K) {
+    MxBwdPlan p;
+    p.n8 = (N + 7) / 8 * 8;
+    p.n64 = (N + 63) / 64 * 64;
+    p.k8 = (K + 7) / 8 * 8;
+    p.pad = dtype == SGCLIP_DTYPE_F32 || N % 64 != 0 || lddy % 8 != 0 || lddy > 0x7fffffff || ((uintptr_t)dy & 15);
+    p.crop = p.n8 != N || p.k8 != K;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align_up(bytes, 256);
+        return here;
+    };
+    p.zeros = take((size_t)K * 4);
+    p.dy = take(p.pad ? (size_t)M * p.n64 * 2 : 0);
+    p.wt = take((size_t)K * p.n64 * 2);
+    p.x = take((size_t)M * p.k8 * 2);
+    p.dw = take(p.crop ? (size_t)p.n8 * p.k8 * 4 : 0);
+    p.parts = take(sgclip_column_sums_workspace_bytes(M, N));
+    p.total = at;
+    return p;
 }
 
 static int mx_epilogue(const char *who, MxGemm &g, int epilogue, const float *bias, const float *aux, int64_t ldaux, void *out, int64_t ldo,
@@ -925,7 +1017,7 @@ int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void 
 }
 
 size_t sgclip_column_sums_workspace_bytes(int M, int N) {
-    return M <= 0 || N <= 0 ? 0 : (size_t)cs_strips(M) * (size_t)N * sizeof(float);
+    return M <= CS_FEW || N <= 0 ? 0 : (size_t)cs_strips(M) * (size_t)N * sizeof(float);
 }
 
 int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int N, float *out_dev, void *workspace_dev, size_t workspace_bytes,
@@ -935,28 +1027,78 @@ int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int 
         set_error("sgclip_column_sums: bad arguments M=%d N=%d ld=%lld dtype=%d", M, N, (long long)ld, in_dtype);
         return SGCLIP_EINVAL;
     }
-    if (M > 0 && (!workspace_dev || workspace_bytes < sgclip_column_sums_workspace_bytes(M, N))) {
+    const int strips = cs_strips(M);
+    if (strips > 1 && (!workspace_dev || workspace_bytes < sgclip_column_sums_workspace_bytes(M, N))) {
         set_error("sgclip_column_sums: workspace of %zu bytes, %zu needed", workspace_dev ? workspace_bytes : (size_t)0,
                   sgclip_column_sums_workspace_bytes(M, N));
         return SGCLIP_ENOSPC;
     }
-    const int strips = M > 0 ? cs_strips(M) : 0;
-    hipStream_t st = (hipStream_t)stream;
-    float *parts = (float *)workspace_dev;
-    const dim3 grid((unsigned)ceil_div(N, CS_COLS), (unsigned)strips);
-    if (strips) {
-        const size_t size = in_dtype == SGCLIP_DTYPE_F32 ? 4 : 2;
-        const bool vec = N % 8 == 0 && ld * size % 16 == 0 && ((uintptr_t)in_dev & 15) == 0;
-        if (in_dtype == SGCLIP_DTYPE_F32) {
-            if (vec) mx_colsum_strip_kernel<float, true><<<grid, 256, 0, st>>>((const float *)in_dev, ld, M, N, parts);
-            else mx_colsum_strip_kernel<float, false><<<grid, 256, 0, st>>>((const float *)in_dev, ld, M, N, parts);
-        } else {
-            if (vec) mx_colsum_strip_kernel<bf16_t, true><<<grid, 256, 0, st>>>((const bf16_t *)in_dev, ld, M, N, parts);
-            else mx_colsum_strip_kernel<bf16_t, false><<<grid, 256, 0, st>>>((const bf16_t *)in_dev, ld, M, N, parts);
-        }
-    }
-    mx_colsum_join_kernel<<<dim3((unsigned)((N + 63) / 64)), 256, 0, st>>>(parts, strips, N, out_dev);
+    const hipStream_t st = (hipStream_t)stream;
+    if (in_dtype == SGCLIP_DTYPE_F32) mx_launch_colsum((const float *)in_dev, ld, M, N, strips, (float *)workspace_dev, out_dev, st);
+    else mx_launch_colsum((const bf16_t *)in_dev, ld, M, N, strips, (float *)workspace_dev, out_dev, st);
     return launch_check("sgclip_column_sums");
+}
+
+size_t sgclip_mxfp4_linear_bwd_workspace_bytes(const void *dy_dev, int dy_dtype, int64_t lddy, int M, int N, int K) {
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : mx_bwd_plan(dy_dev, dy_dtype, lddy, M, N, K).total;
+}
+
+int sgclip_mxfp4_linear_bwd(const void *dy_dev, int dy_dtype, int64_t lddy, const void *x_codes_dev, const void *x_scales_dev,
+                            const void *w_codes_dev, const void *w_scales_dev, int M, int N, int K, void *dx_dev, int dx_dtype, float *dw_dev,
+                            float *db_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
+    const char *who = "sgclip_mxfp4_linear_bwd";
+    if (!mx_shape_ok(who, M, K) || !mx_shape_ok(who, N, K)) return SGCLIP_EINVAL;
+    const hipStream_t st = (hipStream_t)stream;
+    if (M == 0 || N == 0) {
+        if (dx_dev && dx_dtype == SGCLIP_DTYPE_F32) mx_zero((float *)dx_dev, (long long)M * K, (float *)nullptr, 0, st);
+        if (dx_dev && dx_dtype == SGCLIP_DTYPE_BF16) mx_zero((bf16_t *)dx_dev, (long long)M * K, (bf16_t *)nullptr, 0, st);
+        mx_zero(dw_dev, dw_dev ? (long long)N * K : 0, db_dev, db_dev ? N : 0, st);
+        return launch_check(who);
+    }
+    if (!dy_dev || lddy < N || (dy_dtype != SGCLIP_DTYPE_F32 && dy_dtype != SGCLIP_DTYPE_BF16) ||
+        (dx_dev && dx_dtype != SGCLIP_DTYPE_F32 && dx_dtype != SGCLIP_DTYPE_BF16)) {
+        set_error("%s: bad dy (dtype %d, row stride %lld, N %d) or dx dtype %d", who, dy_dtype, (long long)lddy, N, dx_dtype);
+        return SGCLIP_EINVAL;
+    }
+    if (!mx_storage_ok(who, x_codes_dev, x_scales_dev) || !mx_storage_ok(who, w_codes_dev, w_scales_dev)) return SGCLIP_EINVAL;
+    const MxBwdPlan p = mx_bwd_plan(dy_dev, dy_dtype, lddy, M, N, K);
+    if (!workspace_dev || workspace_bytes < p.total || ((uintptr_t)workspace_dev & 15)) {
+        set_error("%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_dev ? workspace_bytes : (size_t)0, p.total);
+        return SGCLIP_ENOSPC;
+    }
+    unsigned char *ws = (unsigned char *)workspace_dev;
+    float *zeros = (float *)(ws + p.zeros), *sum = p.crop ? (float *)(ws + p.dw) : dw_dev;
+    int rc = SGCLIP_OK;
+    if (db_dev) rc = sgclip_column_sums(dy_dev, dy_dtype, lddy, M, N, db_dev, ws + p.parts, p.total - p.parts, stream);
+    if (rc != SGCLIP_OK || (!dx_dev && !dw_dev)) return rc;
+    mx_zero(sum, dw_dev ? (long long)p.n8 * p.k8 : 0, zeros, dx_dev ? K : 0, st);
+    // dy as the products take it: bf16, aligned rows, whole stages of columns
+    const void *dy = dy_dev;
+    long long ld = lddy;
+    if (p.pad) {
+        const long long blocks = ((long long)M * (p.n64 / 8) + 255) / 256;
+        if (!mx_grid_ok(who, blocks, 256)) return SGCLIP_EINVAL;
+        bf16_t *out = (bf16_t *)(ws + p.dy);
+        if (dy_dtype == SGCLIP_DTYPE_F32) mx_pad_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>((const float *)dy_dev, lddy, M, N, out, p.n64);
+        else mx_pad_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>((const bf16_t *)dy_dev, lddy, M, N, out, p.n64);
+        dy = out;
+        ld = p.n64;
+    }
+    if (dx_dev) {
+        rc = sgclip_mxfp4_dequantize(w_codes_dev, w_scales_dev, N, K, 1, ws + p.wt, p.n64, stream);
+        if (rc == SGCLIP_OK)
+            rc = sgclip_gemm_bf16(dy, (int)ld, ws + p.wt, p.n64, dx_dev, K, M, K, p.n64,
+                                  dx_dtype == SGCLIP_DTYPE_F32 ? SGCLIP_EPI_F32 : SGCLIP_EPI_BIAS_BF16, zeros, nullptr, 0, stream);
+        if (rc != SGCLIP_OK) return rc;
+    }
+    if (dw_dev) {
+        // the codes behind the last column are zeros, so that x reads back as one of whole groups of eight columns
+        rc = sgclip_mxfp4_dequantize(x_codes_dev, x_scales_dev, M, p.k8, 0, ws + p.x, p.k8, stream);
+        if (rc == SGCLIP_OK) rc = sgclip_gemm_tn_bf16(dy, (int)ld, ws + p.x, p.k8, sum, p.k8, p.n8, p.k8, M, stream);
+        if (rc != SGCLIP_OK) return rc;
+        if (p.crop) mx_crop_kernel<<<dim3(mx_grid((long long)N * K)), 256, 0, st>>>(sum, p.k8, N, K, dw_dev);
+    }
+    return launch_check(who);
 }
 
 }  // extern "C"

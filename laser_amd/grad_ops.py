@@ -13,7 +13,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .ops import Mxfp4, _apart, _ptr, _same_device, _stream, dequantize_mxfp4, gemm_bf16
+from .ops import Mxfp4, _apart, _ptr, _same_device, _stream, gemm_bf16
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -276,36 +276,21 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
     if dx_dtype not in (BF16, F32):
         raise ValueError(f"linear_mxfp4_bwd: dx in {dx_dtype}")
     _same_device(dy, xq.data, wq.data)
+    return linear_mxfp4_bwd_at(dy, (*xq.pointers(), *wq.pointers()), xq.rows, wq.rows, xq.cols, dx_dtype, need_dx, need_dw, need_db)
+
+
+def linear_mxfp4_bwd_at(dy: torch.Tensor, operands, M: int, N: int, K: int, dx_dtype: torch.dtype, need_dx: bool, need_dw: bool, need_db: bool):
+    """`linear_mxfp4_bwd`, unchecked, by the addresses of x's codes and scales and of the weight's (on dy's device)."""
+    lib, dev = _lib.load(), dy.device
     dy = dy.contiguous()
-    M, N, K = xq.rows, wq.rows, xq.cols
-    dev = dy.device
-    db = column_sums(dy) if need_db else None
-    if M == 0 or N == 0:
-        return (torch.zeros((M, K), dtype=dx_dtype, device=dev) if need_dx else None,
-                torch.zeros((N, K), dtype=F32, device=dev) if need_dw else None, db)
-    dyb = cast_bf16(dy) if dy.dtype == F32 else dy
-    dx = dw = None
-    Np, Kp = pad64(N), (K + 7) // 8 * 8
-    dyp = dyb
-    if (need_dx and N != Np) or (need_dw and N % 8):
-        dyp = torch.empty((M, Np), dtype=BF16, device=dev)
-        dyp[:, :N] = dyb
-        dyp[:, N:] = 0
-    if need_dx:
-        w_t = dequantize_mxfp4(wq, transpose=True)       # [K, N rounded up to 64], zeros behind N
-        dx = torch.empty((M, K), dtype=dx_dtype, device=dev)
-        if dx_dtype == F32:
-            gemm_bf16(dyp, w_t, dx, _lib.EPI_F32)
-        else:
-            gemm_bf16(dyp, w_t, dx, _lib.EPI_BIAS_BF16, bias=torch.zeros(K, dtype=F32, device=dev))
-    if need_dw:
-        # in whole groups of eight columns, as the product takes them from memory: the codes behind the last column are zeros, and
-        # what they and dy's padding give is dropped
-        x = dequantize_mxfp4(Mxfp4(xq.data, M, Kp))
-        if N % 8 == 0 and K == Kp:
-            dw = linear_wgrad(dyb, x)
-        else:
-            dw = linear_wgrad(dyb if N % 8 == 0 else dyp[:, :(N + 7) // 8 * 8], x)[:N, :K].contiguous()
+    dx = torch.empty((M, K), dtype=dx_dtype, device=dev) if need_dx else None
+    dw = torch.empty((N, K), dtype=F32, device=dev) if need_dw else None
+    db = torch.empty(N, dtype=F32, device=dev) if need_db else None
+    head = (dy.data_ptr(), _dtype_code(dy), N)
+    need = lib.sgclip_mxfp4_linear_bwd_workspace_bytes(*head, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.check(lib.sgclip_mxfp4_linear_bwd(*head, *operands, M, N, K, _ptr(dx), _lib.DTYPE_F32 if dx_dtype == F32 else _lib.DTYPE_BF16,
+                                           _ptr(dw), _ptr(db), _ptr(ws), need, _stream(dy)))
     return dx, dw, db
 
 

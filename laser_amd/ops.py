@@ -444,6 +444,34 @@ def dequantize_mxfp4(q: Mxfp4, transpose: bool = False) -> torch.Tensor:
     return out
 
 
+def linear_mxfp4_both(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+    """x [M, K] and weight [N, K] (bf16 / f32) quantised, and their product bf16 [M, N]: (product, bytes of both, offsets of x's codes
+    and scales and of the weight's in them)."""
+    lib = _lib.load()
+    ldx, ldw = _rows2d("linear_mxfp4: x", x, _MX_DTYPES), _rows2d("linear_mxfp4: weight", weight, _MX_DTYPES)
+    (M, K), N = x.shape, weight.shape[0]
+    if K == 0 or weight.shape[1] != K:
+        raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    _check_bias(bias, N)
+    _same_device(x, weight, bias)
+    xc, xs = Mxfp4.sizes(M, K)
+    wc, ws = Mxfp4.sizes(N, K)
+    offsets = (0, xc, xc + xs, xc + xs + wc)
+    data = torch.empty(xc + xs + wc + ws, dtype=torch.uint8, device=x.device)
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    base, stream = data.data_ptr(), _stream(x)
+    at = [base + o for o in offsets]
+    _lib.check(lib.sgclip_mxfp4_quantize(x.data_ptr(), _MX_DTYPES[x.dtype], ldx, M, K, at[0], at[1], stream))
+    _lib.check(lib.sgclip_mxfp4_quantize(weight.data_ptr(), _MX_DTYPES[weight.dtype], ldw, N, K, at[2], at[3], stream))
+    _lib.check(lib.sgclip_mxfp4_gemm(*at, M, N, K, _lib.EPI_BIAS_BF16, _ptr(bias), None, 0, out.data_ptr(), N, stream))
+    return out, data, offsets
+
+
+def _check_bias(bias: Optional[torch.Tensor], N: int):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"linear_mxfp4: bias must be contiguous f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+
+
 def linear_mxfp4(x, w: Mxfp4, bias: Optional[torch.Tensor] = None, *, gelu: bool = False, residual: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x w^T + bias with both operands in 4-bit floats and fp32 sums.  x: bf16 / f32 [M, K], quantised on the way, or an Mxfp4;
@@ -458,8 +486,7 @@ def linear_mxfp4(x, w: Mxfp4, bias: Optional[torch.Tensor] = None, *, gelu: bool
     if K != w.cols:
         raise ValueError(f"linear_mxfp4: x has {K} columns, the weight {w.cols}")
     dtype, epi, ldr = torch.bfloat16, _lib.EPI_BIAS_GELU_BF16 if gelu else _lib.EPI_BIAS_BF16, 0
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
-        raise ValueError(f"linear_mxfp4: bias must be contiguous f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+    _check_bias(bias, N)
     if residual is not None:
         if gelu:
             raise ValueError("linear_mxfp4: gelu and residual exclude each other")

@@ -506,18 +506,19 @@ def segment_mean(probs: torch.Tensor, seg: torch.Tensor, n_groups: int, seg_host
 class _LinearMxfp4Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(weight)
-        ctx.save_for_backward(xq.data, wq.data)
-        ctx.shapes, ctx.dtypes = (xq.shape, wq.shape), (x.dtype, weight.dtype)
-        return ops.linear_mxfp4(xq, wq, bias)
+        y, data, ctx.offsets = ops.linear_mxfp4_both(x, weight, bias)
+        ctx.save_for_backward(data)
+        ctx.dims, ctx.dtypes = (x.shape[0], weight.shape[0], x.shape[1]), (x.dtype, weight.dtype)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("linear_mxfp4's backward is not captured: call grad_ops.linear_mxfp4_bwd")
-        xq, wq = (ops.Mxfp4(data, *shape) for data, shape in zip(ctx.saved_tensors, ctx.shapes))
-        dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, ctx.dtypes[0], *ctx.needs_input_grad)
+        data, = ctx.saved_tensors
+        base = data.data_ptr()
+        dx, dw, db = G.linear_mxfp4_bwd_at(dy, [base + at for at in ctx.offsets], *ctx.dims, ctx.dtypes[0], *ctx.needs_input_grad)
         return dx, dw if dw is None else dw.to(ctx.dtypes[1]), db
 
 

@@ -296,6 +296,36 @@ def test_gradients_against_64_bits(M, N, K, dtype):
     _check(db, eb, sb, M, 0)
 
 
+@pytest.mark.parametrize("M,N,K", [(513, 1032, 131), (1000, 517, 64), (9000, 96, 250)])
+def test_gradients_of_f32_and_strided_dy(M, N, K):
+    xq, wq = ops.quantize_mxfp4(_x(M, K, BF16)), ops.quantize_mxfp4(0.05 * torch.randn(N, K, device="cuda"))
+    xv, wv = ops.dequantize_mxfp4(xq).double(), ops.dequantize_mxfp4(wq).double()
+    for dy in (torch.randn(M, N, device="cuda"), torch.randn(M, N + 3, device="cuda")[:, 3:], torch.randn(M, N + 8, device="cuda").to(BF16)[:, 8:],
+               torch.randn(M * N + 1, device="cuda").to(BF16)[1:].view(M, N)):
+        d, r = dy.double(), dy.to(BF16).double()
+        dx, dw, db = G.linear_mxfp4_bwd(dy, xq, wq, F32)
+        _check(dx, r @ wv, r.abs() @ wv.abs(), N, 0)
+        _check(dw, r.t() @ xv, r.abs().t() @ xv.abs(), M, 0)
+        _check(db, d.sum(0), d.abs().sum(0), M, 0)
+        for need in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+            got = G.linear_mxfp4_bwd(dy, xq, wq, F32, *need)
+            assert [t is not None for t in got] == list(need)
+            for t, whole in zip(got, (dx, dw, db)):
+                assert t is None or torch.equal(t, whole) or (whole is dw and (t - dw).abs().max() <= 2 * M * U32 * (r.abs().t() @ xv.abs()).max())
+
+
+def test_saved_operands_may_move():
+    """Hooks that keep what forward saved elsewhere: backward finds it where they bring it back."""
+    x, w = torch.randn(70, 96, device="cuda", requires_grad=True), torch.randn(40, 96, device="cuda", requires_grad=True)
+    b = torch.randn(40, device="cuda", requires_grad=True)
+    dy = torch.randn(70, 40, device="cuda").to(BF16)
+    want = torch.autograd.grad(training.linear_mxfp4(x, w, b), (x, w, b), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = training.linear_mxfp4(x, w, b)
+    for got, t in zip(torch.autograd.grad(y, (x, w, b), dy), want):
+        assert torch.allclose(got, t, rtol=1e-5, atol=1e-5 * t.abs().max().item())
+
+
 def test_gradients_against_differences():
     """y is linear in each quantised operand: a difference along any direction is the gradient's inner product exactly (64 bits)."""
     M, N, K = 40, 24, 96

@@ -73,3 +73,23 @@ def test_reference_values():
     want = [4, 0, 0.5, 1, 1, 2, 2, 4, -1, 3, 3, 0, -4, 1, 3, 0.5]
     got = values(x)
     assert got[0, :16].tolist() == want and got[0, 32:34].tolist() == [6, 4]
+
+
+def test_gradient_entry_point(lib):
+    p, E = 4096, _lib.EINVAL
+    need = lib.sgclip_mxfp4_linear_bwd_workspace_bytes
+    # zeros [K], w^T [K][64], x [M][K]; what has to be laid out or cropped comes on top
+    plain = 256 + 64 * 64 * 2 + 40 * 64 * 2
+    assert need(p, _lib.DTYPE_BF16, 64, 40, 64, 64) == plain
+    for dy, dtype, ld in ((p, _lib.DTYPE_F32, 64), (p + 8, _lib.DTYPE_BF16, 64), (p, _lib.DTYPE_BF16, 68)):
+        assert need(dy, dtype, ld, 40, 64, 64) == plain + 40 * 64 * 2
+    assert need(p, _lib.DTYPE_BF16, 61, 40, 61, 64) == plain + 40 * 64 * 2 + 64 * 64 * 4
+    assert need(p, _lib.DTYPE_BF16, 64, 1000, 64, 64) == 256 + 64 * 64 * 2 + 1000 * 64 * 2 + 32 * 64 * 4     # strips of column sums
+    assert need(p, _lib.DTYPE_BF16, 64, 0, 64, 64) == need(p, _lib.DTYPE_BF16, 0, 5, 0, 64) == 0
+
+    def bwd(dy=p, dtype=_lib.DTYPE_BF16, ld=64, xc=p, ws=p, M=40, N=64, K=64, dx=p, dxt=_lib.DTYPE_BF16, dw=p, work=p, size=1 << 20):
+        return lib.sgclip_mxfp4_linear_bwd(dy, dtype, ld, xc, p, p, ws, M, N, K, dx, dxt, dw, p, work, size, None)
+    for bad in (dict(dy=None), dict(dtype=7), dict(ld=63), dict(xc=None), dict(ws=p + 4), dict(M=-1), dict(K=0), dict(dxt=7)):
+        assert bwd(**bad) == E and lib.sgclip_last_error(), bad
+    for bad in (dict(work=None), dict(work=p + 8), dict(size=100)):
+        assert bwd(**bad) == _lib.ENOSPC
