@@ -211,18 +211,47 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
 #pragma unroll
     for (int i = 0; i < SM; i++)
 #pragma unroll
-        for (int j = 0; j < SN; j++) {
-            acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if constexpr (EPI == OR_POLY) {
-                const int m = mw + i * 16 + r, n = nw + j * 16 + q * 4;
-                if (m < g.M && n < or_chunks(g.N) * 32) {
-                    const unsigned char *a = g.A + b * g.sA + m * ldn + or_unit(n);
-                    const f16x4 ah = *(const f16x4 *)a, al = *(const f16x4 *)(a + 64);
+        for (int j = 0; j < SN; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if constexpr (EPI == OR_POLY) {
+        auto init = [&](f32x4 &v, f16x4 hi, f16x4 lo, int m, int n) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] = g.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? g.ca : 0.f);
+            for (int e = 0; e < 4; e++) v[e] = g.cb * ((float)hi[e] + (float)lo[e]) + (m == n + e ? g.ca : 0.f);
+        };
+        const int npad = or_chunks(g.N) * 32;
+#pragma unroll
+        for (int i = 0; i < SM; i++) {
+            const int m = mw + i * 16 + r;
+            const unsigned char *a = g.A + b * g.sA + min(m, g.M - 1) * ldn;
+            if constexpr (SN % 2 == 0) {
+                // 32 columns, eight a lane; then neighbouring rows of 16 lanes, and halves of the wave, exchange to four of each 16
+                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+                for (int j = 0; j < SN; j += 2) {
+                    u32x2 w[2][2];      // block j, j + 1; hi, lo
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const u32x4 v = *(const u32x4 *)(a + or_unit(min(nw + j * 16, npad - 32)) + h * 64 + q * 16);
+#pragma unroll
+                        for (int d = 0; d < 2; d++) {
+                            const u32x2 x = __builtin_amdgcn_permlane16_swap(v[d], v[d + 2], false, false);
+                            const u32x2 y = __builtin_amdgcn_permlane32_swap(x[0], x[1], false, false);
+                            w[0][h][d] = y[0];
+                            w[1][h][d] = y[1];
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) init(acc[i][j + k], __builtin_bit_cast(f16x4, w[k][0]), __builtin_bit_cast(f16x4, w[k][1]), m, nw + (j + k) * 16 + q * 4);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < SN; j++) {
+                    const unsigned char *p = a + or_unit(min(nw + j * 16, npad - 16) + q * 4);
+                    init(acc[i][j], *(const f16x4 *)p, *(const f16x4 *)(p + 64), m, nw + j * 16 + q * 4);
                 }
             }
         }
+    }
     // a row 16 further has the same chunk order
     auto at = [](int bytes, int row, int chunk) { return bytes == 128 ? lds_off(row, chunk) : row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4); };
     const int lh0 = at(LB, wm * SM * 16 + r, q), ll0 = at(128, wm * SM * 16 + r, 4 + q);
