@@ -387,6 +387,14 @@ class Mxfp4:
                              f"{tuple(data.shape)} on {data.device}")
         self.data, self.rows, self.cols, self.split = data, rows, cols, codes
 
+    @classmethod
+    def _allocate(cls, rows: int, cols: int, device) -> "Mxfp4":
+        """Uninitialised storage, which needs none of the constructor's checks."""
+        q = cls.__new__(cls)
+        codes, scales = cls.sizes(rows, cols)
+        q.data, q.rows, q.cols, q.split = torch.empty(codes + scales, dtype=torch.uint8, device=device), rows, cols, codes
+        return q
+
     @staticmethod
     def sizes(rows: int, cols: int):
         """Bytes of the codes and of the scales (sgclip_mxfp4_codes_bytes, sgclip_mxfp4_scales_bytes)."""
@@ -426,8 +434,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     rows, cols = x.shape
     if cols == 0:
         raise ValueError("quantize_mxfp4: rows of no elements")
-    codes, scales = Mxfp4.sizes(rows, cols)
-    q = Mxfp4(torch.empty(codes + scales, dtype=torch.uint8, device=x.device), rows, cols)
+    q = Mxfp4._allocate(rows, cols, x.device)
     p, s = q.pointers()
     _lib.check(_lib.load().sgclip_mxfp4_quantize(x.data_ptr(), _MX_DTYPES[x.dtype], ld, rows, cols, p, s, _stream(x)))
     return q
