@@ -469,7 +469,10 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
 // The stages of a workgroup's tiles form one stream through two LDS slots; a stage is two 128-deep sub-steps whose fragments are
 // double-buffered in registers, with one barrier between them: there every wave holds all of stage g, stage g + 1 has landed,
 // and the DMA of stage g + 2 (of the next tile, if need be) starts into the slot just freed.  A tile's results leave from the registers
-// while the next tile's operands arrive; the barrier after them waits for the fetches only (they are older than the stores, and the counter retires in order).
+// while the next tile's operands arrive; the barrier after them waits for the fetches only (they are older than the stores, and the
+// counter retires in order).
+// 73856 x 1024 x 4096 in 213 us (with GELU 244): 117 are the main loop alone (1.40 a stage, 1.08 at the matrix rate), 25 its fetches, the
+// rest the results, 3.7 a tile (GELU 5.4), behind which the next tile's fetches wait.  K = 4096: 612 us, 4.0 PFLOP/s.
 // ---------------------------------------------------------------------------
 constexpr int MXP_OP = 256 * 128, MXP_SLOT = 2 * MXP_OP + 4096, MXP_BIAS = 2 * MXP_SLOT, MXP_LDS = MXP_BIAS + 4096;
 static_assert(MXP_LDS <= 160 * 1024, "LDS of a CU");

@@ -159,9 +159,11 @@ __device__ __forceinline__ void or_symmetrize(f32x4 &v, unsigned char *region, i
 // columns.  Fragments roll through one set of registers: those of L arrive a few products before their use and are replaced, hi
 // by lo, row by row; in the middle of the last product every wave holds the rest of the stage, the next stage has landed (the
 // one barrier), and the DMA of stage s + SLOTS starts into the slot just freed.
-//   256 x 256: eight waves, 243 registers, 16.1 results per cycle and CU of 21.3 the matrix pipe could do;
-//   192 x 192: eight waves, three slots; 128 x 128: four waves, two workgroups on a CU; both spend 89 - 100 % of the LDS's cycles;
+//   256 x 256: eight waves, 246 registers, 16.1 results per cycle and CU of 21.3 the matrix pipe could do;
+//   192 x 192: eight waves, three slots; 128 x 128: four waves, two workgroups on a CU;
 //   64 x 64: four waves, four slots, for few tiles, where a stage is shorter than its fetch.
+// Bound by the matrix pipe and the fetches beside it (two 128 x 128 tiles on a CU: 2360 cycles a stage, 1500 without fetches, 1536
+// at the matrix rate); the LDS is read half of the time.
 template <int EPI, int FORM, int WM, int WN, int SM, int SN, int SLOTS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
     constexpr int W = WM * WN, T = WM * SM * 16, LB = FORM == OR_PLAIN_L ? 64 : 128, RB = FORM == OR_PLAIN_R ? 64 : 128;   // bytes of a row's stage
@@ -241,7 +243,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < 2; k++) init(acc[i][j + k], __builtin_bit_cast(f16x4, w[k][0]), __builtin_bit_cast(f16x4, w[k][1]), m, nw + (j + k) * 16 + q * 4);
+                    for (int k = 0; k < 2; k++)
+                        init(acc[i][j + k], __builtin_bit_cast(f16x4, w[k][0]), __builtin_bit_cast(f16x4, w[k][1]), m, nw + (j + k) * 16 + q * 4);
                 }
             } else {
 #pragma unroll
@@ -699,8 +702,8 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
     }
     // 64 x 64 tiles where 128 x 128 do not give every CU one (two of 127 x 255: 104 us, with 128 x 128 151 us).  Otherwise the tile whose
     // rounds over the chip cost least: cycles of a stage measured at 1024 x 4096 and 768 x 768, 4080 for a 256 x 256 tile, 2400 for
-    // 192 x 192, 2330 for two 128 x 128 tiles that share a CU (16.1, 15.4 and 14.1 results per cycle: the larger the tile, the less LDS
-    // traffic per product).  48 of 768 x 768: 192 where X is written (3 rounds), 128 on the triangles; 24 of 1024 x 4096: 256.
+    // 192 x 192, 2330 for two 128 x 128 tiles that share a CU (16.1, 15.4 and 14.1 results per cycle: the larger the tile, the fewer
+    // bytes fetched per product).  48 of 768 x 768: 192 where X is written (3 rounds), 128 on the triangles; 24 of 1024 x 4096: 256.
     const int cus = device_cus();
     constexpr bool HALF = FORM == OR_PLAIN_L || FORM == OR_PLAIN_R;     // smaller stages: three slots instead of two
     if (tiles(128) * products < cus) return or_launch_tile<EPI, FORM, 2, 2, 2, 2, 4>(g, tiles(64), products, stream);
