@@ -38,6 +38,7 @@ typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int OR_BATCH = 64;      // matrices per launch: their pointers travel as kernel arguments
 constexpr int OR_PARTS = 64;      // partial sums of a matrix's squared norm
+constexpr int OR_STEPS = 32;
 
 static __host__ __device__ inline int or_chunks(int k) { return (k + 31) / 32; }
 static __host__ __device__ inline int or_split_ld(int k) { return (k + 31) / 32 * 128; }
@@ -47,7 +48,10 @@ struct OrPointers {
     void *p[OR_BATCH];
 };
 
+// The statement between: where v is a product in the compiler's sight, it rounds that to hi once in one place and by way of fp32 in
+// another, and now and then lo belongs to a neighbour of hi (one element in 2^17 off by 2^-11).
 __device__ __forceinline__ void or_split(float v, f16_t &hi, f16_t &lo) {
+    asm("" : "+v"(v));
     hi = (f16_t)v;
     lo = (f16_t)(v - (float)hi);
 }
@@ -605,6 +609,256 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
 }
 
 // ---------------------------------------------------------------------------
+// Small matrices: the whole step of one matrix in one workgroup, where a chain of launches would cost more than its products.
+// A wave keeps 16 columns of X (m <= 16 MT rows) in registers, from step to step.  They lie there as the matrix instruction leaves a
+// result and, with the columns of M in the same order (32 of them: four of the first 16, then four of the second), takes its
+// second operand, so that M X needs nothing of X but registers.  For A = X X^T the waves lay out X's rows in LDS, then A, then M; the
+// lower 16 x 16 tiles of A and M are computed and written to both sides.
+// Bound by one CU: 128 x 256 take 3.5 us a step on its matrix pipe and as long to read their fragments from LDS, between five
+// barriers.  Against the launches of or_gemm_kernel, us: 4 of 33 x 64 19 (67), of 64 x 64 20 (68), of 65 x 255 41 (85), of 128 x 128 47
+// (79), of 127 x 255 67 (86); 200 of them 291 (442).
+// ---------------------------------------------------------------------------
+struct OrSmall {
+    OrInput in;
+    OrPointers out;
+    long long ldo;
+    int m, n, flip, steps;
+    float scale, eps, decay, rate;
+    struct {
+        float gram, ca, cb, poly, apply;     // A = gram X X^T, M = poly (ca I + cb A + A A), X = apply M X
+        int square;                          // 0: without A A
+    } s[OR_STEPS];
+};
+
+// A and M, MT tiles wide: 16-byte units of a row, hi then lo
+template <int MT>
+struct OrSmallRows {
+    static constexpr int UNITS = MT > 4 ? 16 : 8, LO = UNITS * 16, ROW = 2 * LO, REGION = MT * 16 * ROW;
+    // where the four elements of row from column col lie
+    static __device__ __forceinline__ int at(int row, int col) {
+        return row * ROW + ((((col >> 5) * 4 + ((col & 15) >> 2)) ^ (row & (UNITS - 1))) << 4) + ((col >> 4) & 1) * 8;
+    }
+};
+
+// Four neighbouring lanes' four values each, transposed: lane s of the four gets value s of all of them.
+__device__ __forceinline__ f16x4 or_transpose4(f16x4 v, int lane) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const bool upper = lane & 2, odd = lane & 1;
+    const unsigned keep = upper ? w[1] : w[0];
+    const unsigned got = __builtin_amdgcn_update_dpp(0, upper ? w[0] : w[1], 0x4e, 0xf, 0xf, true);      // quad_perm 2 3 0 1
+    const unsigned a = upper ? got : keep, b = upper ? keep : got;                                       // of the lower and of the upper pair
+    const unsigned first = 0x05040100u, second = 0x07060302u;
+    const unsigned mine = __builtin_amdgcn_perm(b, a, odd ? second : first);
+    const unsigned other = __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_perm(b, a, odd ? first : second), 0xb1, 0xf, 0xf, true);   // 1 0 3 2
+    return __builtin_bit_cast(f16x4, (u32x2){__builtin_amdgcn_perm(other, mine, odd ? 0x01000504u : first),
+                                             __builtin_amdgcn_perm(other, mine, odd ? 0x03020706u : second)});
+}
+
+// a lane's four results, row i 16 + r, columns j 16 + q 4 .., and the same across the diagonal
+template <int MT>
+__device__ __forceinline__ void or_small_store(unsigned char *base, const f32x4 &v, int i, int j, int lane) {
+    using Rows = OrSmallRows<MT>;
+    const int r = lane & 15, q = lane >> 4;
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        f16_t h, l;
+        or_split(v[e], h, l);
+        hi[e] = h;
+        lo[e] = l;
+    }
+    unsigned char *p = base + Rows::at(i * 16 + r, j * 16 + q * 4);
+    *(f16x4 *)p = hi;
+    *(f16x4 *)(p + Rows::LO) = lo;
+    if (i == j) return;
+    p = base + Rows::at(j * 16 + q * 4 + (r & 3), i * 16 + (r >> 2) * 4);
+    *(f16x4 *)p = or_transpose4(hi, lane);
+    *(f16x4 *)(p + Rows::LO) = or_transpose4(lo, lane);
+}
+
+// hi hi, then hi lo and lo hi
+__device__ __forceinline__ void or_small_multiply(f32x4 &big, f32x4 &small, f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl) {
+    big = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, big, 0, 0, 0);
+    small = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, small, 0, 0, 0);
+    small = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, small, 0, 0, 0);
+}
+
+// `count` of four elements `step` apart (the others zeros); four side by side in one access of any alignment
+template <typename T>
+__device__ __forceinline__ f32x4 or_small_load(const T *p, long long step, int count) {
+    typedef T any4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (step == 1 && count == 4) {
+        const any4 w = *(const any4 *)p;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (float)w[e];
+        return v;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < count) v[e] = (float)p[e * step];
+    return v;
+}
+
+template <typename T, typename V>
+__device__ __forceinline__ void or_small_write(T *p, long long step, int count, V v) {
+    typedef T any4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (step == 1 && count == 4) {
+        *(any4 *)p = (any4){v[0], v[1], v[2], v[3]};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < count) p[e * step] = v[e];
+}
+
+template <typename T, bool STEP, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    __shared__ double wsum[NW];
+    using Rows = OrSmallRows<MT>;
+    constexpr int XROW = NW * 64, XLO = XROW / 2, NT = MT * (MT + 1) / 2, TILES = (NT + NW - 1) / NW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const int n = wave * 16 + r;
+    f32x4 x[MT];
+    double sum = 0.0;
+    const T *g = (const T *)a.in.g.p[blockIdx.x];
+    float *buf = (float *)a.in.buf.p[blockIdx.x];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = i * 16 + q * 4, count = n < a.n ? min(max(a.m - m, 0), 4) : 0;
+        x[i] = or_small_load(g + (a.flip ? n * a.in.ldg + m : m * a.in.ldg + n), a.flip ? 1 : a.in.ldg, count);
+        if constexpr (STEP) {
+            float *bp = buf + (a.flip ? (long long)n * a.in.cols + m : (long long)m * a.in.cols + n);
+            const long long step = a.flip ? 1 : a.in.cols;
+            f32x4 b = or_small_load(bp, step, count);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                b[e] = a.in.mu * b[e] + (1.0f - a.in.mu) * x[i][e];
+                x[i][e] = or_direction<T, STEP>(a.in, x[i][e], b[e]);
+            }
+            or_small_write(bp, step, count, b);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += (double)x[i][e] * x[i][e];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) wsum[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) sum += wsum[w];
+    const double inv = (double)a.scale / (sqrt(sum) + (double)a.eps);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i][e] = (float)(x[i][e] * inv);
+
+    // the wave's tiles of the lower triangle, row by row
+    int ti[TILES], tj[TILES];
+#pragma unroll
+    for (int k = 0; k < TILES; k++) {
+        const int t = wave + k * NW;
+        ti[k] = (t >= 1) + (t >= 3) + (t >= 6) + (t >= 10) + (t >= 15) + (t >= 21) + (t >= 28);
+        tj[k] = t - ti[k] * (ti[k] + 1) / 2;
+    }
+    const int sw = r & (Rows::UNITS - 1);
+    for (int s = 0; s < a.steps; s++) {
+        f16x8 xh[MT / 2], xl[MT / 2];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            f16x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f16_t h, l;
+                or_split(x[i][e], h, l);
+                hi[e] = xh[i / 2][i % 2 * 4 + e] = h;
+                lo[e] = xl[i / 2][i % 2 * 4 + e] = l;
+            }
+            const int row = i * 16 + q * 4 + (r & 3);
+            unsigned char *p = lds + row * XROW + (((wave * 2 + (r >> 3)) ^ (row & 15)) << 4) + ((r >> 2) & 1) * 8;
+            *(f16x4 *)p = or_transpose4(hi, lane);
+            *(f16x4 *)(p + XLO) = or_transpose4(lo, lane);
+        }
+        __syncthreads();
+        f32x4 t[TILES];
+#pragma unroll
+        for (int k = 0; k < TILES; k++) {
+            t[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (wave + k * NW >= NT) continue;
+            const unsigned char *left = lds + (ti[k] * 16 + r) * XROW, *right = lds + (tj[k] * 16 + r) * XROW;
+            f32x4 small = t[k];
+#pragma unroll
+            for (int c = 0; c < NW / 2; c++) {
+                const int u = ((c * 4 + q) ^ r) << 4;
+                or_small_multiply(t[k], small, *(const f16x8 *)(right + u), *(const f16x8 *)(right + XLO + u), *(const f16x8 *)(left + u),
+                                  *(const f16x8 *)(left + XLO + u));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) t[k][e] = (t[k][e] + small[e]) * a.s[s].gram;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TILES; k++)
+            if (wave + k * NW < NT) or_small_store<MT>(lds, t[k], ti[k], tj[k], lane);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TILES; k++) {
+            if (wave + k * NW >= NT) continue;
+            f32x4 v, small = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = a.s[s].cb * t[k][e] + (ti[k] == tj[k] && q * 4 + e == r ? a.s[s].ca : 0.f);
+            if (a.s[s].square) {
+                const unsigned char *left = lds + (ti[k] * 16 + r) * Rows::ROW, *right = lds + (tj[k] * 16 + r) * Rows::ROW;
+#pragma unroll
+                for (int c = 0; c < MT / 2; c++) {
+                    const int u = ((c * 4 + q) ^ sw) << 4;
+                    or_small_multiply(v, small, *(const f16x8 *)(right + u), *(const f16x8 *)(right + Rows::LO + u), *(const f16x8 *)(left + u),
+                                      *(const f16x8 *)(left + Rows::LO + u));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (v[e] + small[e]) * a.s[s].poly;
+            or_small_store<MT>(lds + Rows::REGION, v, ti[k], tj[k], lane);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f}, small = v;
+            const unsigned char *left = lds + Rows::REGION + (i * 16 + r) * Rows::ROW;
+#pragma unroll
+            for (int c = 0; c < MT / 2; c++) {
+                const int u = ((c * 4 + q) ^ sw) << 4;
+                or_small_multiply(v, small, *(const f16x8 *)(left + u), *(const f16x8 *)(left + Rows::LO + u), xh[c], xl[c]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][e] = (v[e] + small[e]) * a.s[s].apply;
+            if constexpr (MT * NW > 64) __builtin_amdgcn_sched_barrier(0);     // or too many fragments are read ahead for the registers
+        }
+        __syncthreads();     // before the next step's X takes the place of M
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = i * 16 + q * 4, count = n < a.n ? min(max(a.m - m, 0), 4) : 0;
+        const long long at = a.flip ? n * a.ldo + m : m * a.ldo + n, step = a.flip ? 1 : a.ldo;
+        if constexpr (STEP) {
+            float *o = (float *)a.out.p[blockIdx.x] + at;
+            f32x4 p = or_small_load(o, step, count);
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] = p[e] * a.decay - a.rate * x[i][e];
+            or_small_write(o, step, count, p);
+        } else {
+            bf16x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (bf16_t)x[i][e];
+            or_small_write((bf16_t *)a.out.p[blockIdx.x] + at, step, count, v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 struct OrPlan {
@@ -636,8 +890,6 @@ struct OrStep {
     double a, b, c;
     int em, et, ea;     // exponents of M = p(A), of T = A M and of A' = M A M
 };
-
-constexpr int OR_STEPS = 32;
 
 // The steps' blocks and exponents from bounds over the range of singular values.
 struct OrSchedule {
@@ -718,11 +970,69 @@ static int or_launch(const OrGemm &gin, int batch, int products, hipStream_t str
 
 static inline float or_pow2(int e) { return ldexpf(1.0f, e); }
 
+// M = p(A) in the accumulators' scale: alpha (ca I + cb A + A A), for A scaled by 2^ea and M by 2^em.  A coefficient c below the
+// rounding of the others' terms is none: then nothing is multiplied.
+struct OrPoly {
+    float alpha, ca, cb;
+    bool square;
+};
+
+static OrPoly or_poly(const OrStep &s, int ea) {
+    OrPoly p;
+    p.square = fabs(s.c) > 1e-12 * fmax(fabs(s.a), fabs(s.b));
+    const double c = p.square ? ldexp(s.c, s.em - 2 * ea) : 1.0;
+    p.alpha = (float)c;
+    p.ca = (float)(ldexp(s.a, s.em) / c);
+    p.cb = (float)(ldexp(s.b, s.em - ea) / c);
+    return p;
+}
+
+template <typename T, bool STEP, int MT, int NW>
+static int or_launch_small(const OrSmall &a, int batch, hipStream_t stream) {
+    constexpr int X = MT * 16 * NW * 64, AM = 2 * OrSmallRows<MT>::REGION, LDS = X > AM ? X : AM;
+    if (!lds_attr((const void *)or_small_kernel<T, STEP, MT, NW>, LDS)) return SGCLIP_ELAUNCH;
+    or_small_kernel<T, STEP, MT, NW><<<dim3(batch), 64 * NW, LDS, stream>>>(a);
+    return launch_check("sgclip_orthogonalize");
+}
+
+// Up to 128 x 256, step by step.
+template <typename T, bool STEP>
+static int or_run_small(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
+                        hipStream_t stream) {
+    OrSmall a{};
+    a.in = in;
+    a.out = out;
+    a.ldo = ldo;
+    a.flip = in.rows > in.cols;
+    a.m = a.flip ? in.cols : in.rows;
+    a.n = a.flip ? in.rows : in.cols;
+    a.steps = sch.steps;
+    a.scale = or_pow2(sch.ex[0]);
+    a.eps = eps;
+    a.decay = decay;
+    a.rate = rate;
+    for (int k = 0; k < sch.steps; k++) {
+        const OrStep &s = sch.s[k];
+        const OrPoly p = or_poly(s, sch.ea0[k]);
+        a.s[k].gram = or_pow2(sch.ea0[k] - 2 * sch.ex[k]);
+        a.s[k].ca = p.ca;
+        a.s[k].cb = p.cb;
+        a.s[k].poly = p.alpha;
+        a.s[k].square = p.square;
+        a.s[k].apply = or_pow2((k + 1 < sch.steps ? sch.ex[k + 1] : 0) - s.em - sch.ex[k]);
+    }
+    if (a.m <= 64) return a.n <= 128 ? or_launch_small<T, STEP, 4, 8>(a, batch, stream) : or_launch_small<T, STEP, 4, 16>(a, batch, stream);
+    if (a.m <= 96) return a.n <= 128 ? or_launch_small<T, STEP, 6, 8>(a, batch, stream) : or_launch_small<T, STEP, 6, 16>(a, batch, stream);
+    return a.n <= 128 ? or_launch_small<T, STEP, 8, 8>(a, batch, stream) : or_launch_small<T, STEP, 8, 16>(a, batch, stream);
+}
+
 // One launch group of up to OR_BATCH matrices.  in: gradients (and momentum buffers); out: bf16 results or parameters.
 template <typename T, bool STEP>
 static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
                   unsigned char *ws, hipStream_t stream) {
     const OrPlan p = or_plan(in.rows, in.cols);
+    // as far as X and the squares fit a CU's LDS and registers; there it is faster at every size and number (above)
+    if (p.m <= 128 && p.n <= 256) return or_run_small<T, STEP>(in, out, ldo, batch, sch, eps, decay, rate, stream);
     unsigned char *X = ws, *XT = X + p.x * batch, *XT2 = XT + p.xt * batch, *A = XT2 + p.xt * batch, *M = A + p.sq * batch, *Tm = M + p.sq * batch,
                   *Q = Tm + p.sq * batch, *Q2 = Q + p.sq * batch;
     double *parts = (double *)(Q2 + p.sq * batch);
@@ -757,13 +1067,11 @@ static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int b
             g.L[0] = g.R = g.A = A;
             unsigned char *Mi = i == 0 ? Q : M;
             g.O[0] = Mi;
-            // a coefficient c below the rounding of the others' terms is none: then nothing is multiplied
-            const bool square = fabs(s.c) > 1e-12 * fmax(fabs(s.a), fabs(s.b));
-            const double c = square ? ldexp(s.c, s.em - 2 * ea) : 1.0;
-            g.alpha[0] = (float)c;
-            g.ca = (float)(ldexp(s.a, s.em) / c);
-            g.cb = (float)(ldexp(s.b, s.em - ea) / c);
-            g.kc = square ? km : 0;
+            const OrPoly poly = or_poly(s, ea);
+            g.alpha[0] = poly.alpha;
+            g.ca = poly.ca;
+            g.cb = poly.cb;
+            g.kc = poly.square ? km : 0;
             if ((rc = or_launch<OR_POLY>(g, batch, 1, stream)) != SGCLIP_OK) break;
             g.kc = km;
             if (i == 0) eq = s.em;

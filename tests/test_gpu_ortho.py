@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 
 BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
 A, B, C2 = G.NEWTON_SCHULZ
-UBF = 2.0 ** -8
+UBF, U32 = 2.0 ** -8, 2.0 ** -24
 BLOCK = abs(B) / A * sum(A ** (2 * k) for k in range(5)) * 2.0 ** -23
 SINGLE = 20 * A ** 5 * 2.0 ** -23
 
@@ -158,6 +158,29 @@ def test_bf16_matrices(batch, rows, cols, steps):
     x = spectrum("strong directions", rows, cols, batch).to(BF16)
     want = iterate(x, steps)
     assert rounded(G.orthogonalize(x, steps=steps), want, tolerance(rows, cols, want / math.sqrt(batch)))
+
+
+@pytest.mark.parametrize("m", [1, 2, 32, 33, 64, 65, 96, 97, 128])
+@pytest.mark.parametrize("n", [1, 5, 64, 100, 128, 129, 200, 255, 256, 257])
+def test_small_matrices(m, n):
+    """What one workgroup holds, and the first sizes beyond it: both orientations, both types, updates with momentum."""
+    for rows, cols in ((m, n), (n, m)):
+        g = spectrum("gaussian", rows, cols, 3)
+        want = iterate(g)
+        tol = tolerance(rows, cols, want / math.sqrt(3))
+        assert rel(raw(g), want) <= tol
+        for dtype in (F32, BF16):
+            assert rel(G.orthogonalize(g.to(dtype)), iterate(g.to(dtype))) <= tol + UBF
+        p, buf = torch.randn(3, rows, cols, device="cuda"), torch.randn(3, rows, cols, device="cuda")
+        mom = 0.9 * buf.double() + 0.1 * g.double()
+        u = 0.1 * g.double() + 0.9 * mom
+        o = iterate(u)
+        wantp = p.double() * (1 - 0.1 * 0.3) - 0.1 * 0.5 * o
+        before = p.double().norm()
+        G.muon_step(list(p), list(g), buf, lr=0.1, momentum=0.9, weight_decay=0.3, scale=0.5)
+        # momentum: three fp32 operations on each element; parameters: the direction's tolerance and three operations
+        assert (buf.double() - mom).norm() <= 4 * U32 * (buf.double().norm() + g.double().norm())
+        assert (p.double() - wantp).norm() <= 0.05 * 2 * tol * o.norm() + 4 * U32 * (before + o.norm())
 
 
 @pytest.mark.parametrize("rows,cols", [(150, 200), (700, 300)])
