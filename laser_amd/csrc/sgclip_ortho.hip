@@ -6,8 +6,8 @@
 //   * several steps need X only once: M_i = p(A_i), Q <- M_i Q, A_{i+1} = M_i A_i M_i, then X <- Q X.  A block of k steps costs
 //     3 m^2 n + (4 k - 3) m^3 multiplications and additions instead of k (3 m^2 n + m^3).
 // The price of a block is precision, since A holds the squares of the singular values: against 64 bits the result of five
-// steps is off by 1e-6 (relative, before its rounding) step by step and by 2e-5 to 1.5e-4 as one block, worst of gaussian, power-law,
-// exponential and low-rank spectra.  Blocks are at most five steps long, and only used where they save time.
+// steps is off by 1e-6 (relative, before its rounding) step by step and by 2e-6 (gaussian matrices) to 3e-4 as one block (power-law,
+// exponential and low-rank spectra).  Blocks are at most five steps long, and only used where they save time.
 //
 // Precision.  The first steps multiply small singular values by a each, 485 times over five steps with the usual coefficients,
 // and rounding errors with them: with bf16 products the result is off by 2 to 20 %, with fp16 by 0.2 to 3 %.  Operands are
