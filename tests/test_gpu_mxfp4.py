@@ -172,6 +172,35 @@ def test_linear_of_any_alignment(M, N, K):
         assert (t == 7.0).all()
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^32 elements: the last rows of each result are those of the last rows alone."""
+    rows, cols, N = 1100000, 4000, 2048
+    base = _x(997, cols, BF16)
+    x = torch.empty((rows, cols), dtype=BF16, device="cuda")
+    for at in range(0, rows, 997):
+        x[at:at + 997] = base[: min(997, rows - at)]
+    x[-64:] = _x(64, cols, BF16)
+    tail = x[-64:].clone()
+    q = ops.quantize_mxfp4(x)
+    assert torch.equal(ops.dequantize_mxfp4(q)[-64:].double(), values(tail))
+    sums, half = G.column_sums(x), x.new_zeros(cols, dtype=F64)
+    for at in range(0, rows, 100000):
+        half += x[at:at + 100000].sum(0, dtype=F64)
+    assert (sums.double() - half).abs().max() <= 2.0 ** -16 * rows * base.abs().max().item()
+    w = ops.quantize_mxfp4(0.02 * torch.randn(N, cols, device="cuda"))
+    want = ops.linear_mxfp4(ops.quantize_mxfp4(tail), w, gelu=True)
+    assert torch.equal(ops.linear_mxfp4(q, w, gelu=True)[-64:], want)
+    assert torch.equal(ops.linear_mxfp4(x, w, gelu=True)[-64:], want)
+    del q
+    out = torch.empty((rows, N + 1), device="cuda")[:, 1:]          # rows that begin anywhere, in one kernel after another
+    for n in (N, 1023):
+        wn = w if n == N else ops.quantize_mxfp4(0.02 * torch.randn(n, cols, device="cuda"))
+        o = out[:, :n]
+        o.zero_()
+        ops.linear_mxfp4(x, wn, residual=o, out=o)
+        assert torch.equal(o[-64:], ops.linear_mxfp4(tail, wn, residual=torch.zeros(64, n, device="cuda")))
+
+
 def test_linear_views_in_place_and_untouched_neighbours():
     M, N, K = 70, 96, 160
     x = _x(2 * M, K + 9, BF16)[::2, 5:5 + K]

@@ -213,6 +213,18 @@ def test_bf16_zero_and_not_finite_matrices_stay_by_themselves():
                 assert rel(y[i], iterate(g[i])) <= 3 * tolerance(rows, cols, iterate(g[i])) + UBF
 
 
+def test_offsets_beyond_32_bits():
+    store = torch.zeros((70, 8200, 8192), dtype=BF16, device="cuda")         # 4.7e9 elements
+    for rows, cols in ((60, 50), (300, 40), (260, 8192)):
+        g = store[:, 7900:7900 + rows, :cols]
+        g.copy_(torch.randn(1, rows, cols, device="cuda"))
+        g[-1] = torch.randn(rows, cols, device="cuda")
+        y = G.orthogonalize(g)
+        assert torch.equal(y[-1], G.orthogonalize(g[-1].contiguous())) and torch.equal(y[0], y[-2])
+        out = store[:, :rows, :cols]
+        assert torch.equal(G.orthogonalize(g.contiguous(), out=out), y)
+
+
 def test_views_outputs_and_neighbours():
     base = torch.randn(5, 90, 140, device="cuda")
     for dtype in (F32, BF16):
