@@ -609,14 +609,19 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
 }
 
 // ---------------------------------------------------------------------------
-// Small matrices: the whole step of one matrix in one workgroup, where a chain of launches would cost more than its products.
+// Matrices of few rows (m <= 128): up to 256 columns the whole step of one matrix in one workgroup, where a chain of launches would
+// cost more than its products; beyond that (WIDE) a workgroup per 256 columns and a launch per step, between which X and each strip's
+// part of X X^T pass through memory; every workgroup adds the parts, in order, and computes p(A) for itself.
 // A wave keeps 16 columns of X (m <= 16 MT rows) in registers, from step to step.  They lie there as the matrix instruction leaves a
 // result and, with the columns of M in the same order (32 of them: four of the first 16, then four of the second), takes its
 // second operand, so that M X needs nothing of X but registers.  For A = X X^T the waves lay out X's rows in LDS, then A, then M; the
 // lower 16 x 16 tiles of A and M are computed and written to both sides.
 // Bound by one CU: 128 x 256 take 3.5 us a step on its matrix pipe and as long to read their fragments from LDS, between five
-// barriers.  Against the launches of or_gemm_kernel, us: 4 of 33 x 64 19 (67), of 64 x 64 20 (68), of 65 x 255 41 (85), of 128 x 128 47
-// (79), of 127 x 255 67 (86); 200 of them 291 (442).
+// barriers.  Against the launches of or_gemm_kernel, us: 4 of 33 x 64 18 (67), of 64 x 64 19 (68), of 65 x 255 39 (85), of 128 x 128 45
+// (79), of 127 x 255 66 (86); 200 of them 284 (442).  In strips: 4 of 64 x 513 46 (89), of 64 x 2000 55 (136), of 96 x 1023 72 (116), of
+// 127 x 513 96 (97), of 127 x 2000 128 (163).
+// A product's results are used in its own block of instructions, never behind a branch beside it: the compiler leaves the wait for the
+// matrix instruction out where a longer path to the same place exists.
 // ---------------------------------------------------------------------------
 struct OrSmall {
     OrInput in;
@@ -624,6 +629,10 @@ struct OrSmall {
     long long ldo;
     int m, n, flip, steps;
     float scale, eps, decay, rate;
+    // WIDE: the launch's place, 0 (X and its Gram matrix) to steps (step s - 1; the last writes the result), and what passes between them
+    int launch;
+    const double *parts;
+    float *x, *gram[2];     // [batch][strips][..]: X as the threads hold it; sums of a strip's part of X X^T, written and read by turns
     struct {
         float gram, ca, cb, poly, apply;     // A = gram X X^T, M = poly (ca I + cb A + A A), X = apply M X
         int square;                          // 0: without A A
@@ -713,48 +722,17 @@ __device__ __forceinline__ void or_small_write(T *p, long long step, int count, 
         if (e < count) p[e * step] = v[e];
 }
 
-template <typename T, bool STEP, int MT, int NW>
+template <typename T, bool STEP, int MT, int NW, bool WIDE>
 __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     __shared__ double wsum[NW];
     using Rows = OrSmallRows<MT>;
     constexpr int XROW = NW * 64, XLO = XROW / 2, NT = MT * (MT + 1) / 2, TILES = (NT + NW - 1) / NW;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
-    const int n = wave * 16 + r;
-    f32x4 x[MT];
-    double sum = 0.0;
-    const T *g = (const T *)a.in.g.p[blockIdx.x];
-    float *buf = (float *)a.in.buf.p[blockIdx.x];
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int m = i * 16 + q * 4, count = n < a.n ? min(max(a.m - m, 0), 4) : 0;
-        x[i] = or_small_load(g + (a.flip ? n * a.in.ldg + m : m * a.in.ldg + n), a.flip ? 1 : a.in.ldg, count);
-        if constexpr (STEP) {
-            float *bp = buf + (a.flip ? (long long)n * a.in.cols + m : (long long)m * a.in.cols + n);
-            const long long step = a.flip ? 1 : a.in.cols;
-            f32x4 b = or_small_load(bp, step, count);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                b[e] = a.in.mu * b[e] + (1.0f - a.in.mu) * x[i][e];
-                x[i][e] = or_direction<T, STEP>(a.in, x[i][e], b[e]);
-            }
-            or_small_write(bp, step, count, b);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) sum += (double)x[i][e] * x[i][e];
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) wsum[wave] = sum;
-    __syncthreads();
-    sum = 0.0;
-#pragma unroll
-    for (int w = 0; w < NW; w++) sum += wsum[w];
-    const double inv = (double)a.scale / (sqrt(sum) + (double)a.eps);
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[i][e] = (float)(x[i][e] * inv);
+    const int strip = WIDE ? blockIdx.x : 0, strips = WIDE ? gridDim.x : 1, b = WIDE ? blockIdx.y : blockIdx.x;
+    const int n = strip * (NW * 16) + wave * 16 + r;
+    f32x4 x[MT], t[TILES];
+    f16x8 xh[MT / 2], xl[MT / 2];
 
     // the wave's tiles of the lower triangle, row by row
     int ti[TILES], tj[TILES];
@@ -765,17 +743,68 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
         tj[k] = t - ti[k] * (ti[k] + 1) / 2;
     }
     const int sw = r & (Rows::UNITS - 1);
-    for (int s = 0; s < a.steps; s++) {
-        f16x8 xh[MT / 2], xl[MT / 2];
+
+    // X = U 2^e / (|U| + eps)
+    auto load = [&]() {
+        const T *g = (const T *)a.in.g.p[b];
+        float *buf = (float *)a.in.buf.p[b];
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int m = i * 16 + q * 4, count = n < a.n ? min(max(a.m - m, 0), 4) : 0;
+            x[i] = or_small_load(g + (a.flip ? n * a.in.ldg + m : m * a.in.ldg + n), a.flip ? 1 : a.in.ldg, count);
+            if constexpr (STEP) {
+                float *bp = buf + (a.flip ? (long long)n * a.in.cols + m : (long long)m * a.in.cols + n);
+                const long long step = a.flip ? 1 : a.in.cols;
+                f32x4 v = or_small_load(bp, step, count);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (!WIDE) v[e] = a.in.mu * v[e] + (1.0f - a.in.mu) * x[i][e];      // (WIDE: done with the norm)
+                    x[i][e] = or_direction<T, STEP>(a.in, x[i][e], v[e]);
+                }
+                if constexpr (!WIDE) or_small_write(bp, step, count, v);
+            }
+            if constexpr (!WIDE) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += (double)x[i][e] * x[i][e];
+            }
+        }
+        if constexpr (WIDE) sum = a.parts[(long long)b * OR_PARTS + lane];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if constexpr (!WIDE) {
+            if (lane == 0) wsum[wave] = sum;
+            __syncthreads();
+            sum = 0.0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) sum += wsum[w];
+        }
+        const double inv = (double)a.scale / (sqrt(sum) + (double)a.eps);
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][e] = (float)(x[i][e] * inv);
+    };
+    auto split = [&]() {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f16_t h, l;
+                or_split(x[i][e], h, l);
+                xh[i / 2][i % 2 * 4 + e] = h;
+                xl[i / 2][i % 2 * 4 + e] = l;
+            }
+    };
+    // X's rows in LDS, and t = X X^T
+    auto gram = [&]() {
 #pragma unroll
         for (int i = 0; i < MT; i++) {
             f16x4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                f16_t h, l;
-                or_split(x[i][e], h, l);
-                hi[e] = xh[i / 2][i % 2 * 4 + e] = h;
-                lo[e] = xl[i / 2][i % 2 * 4 + e] = l;
+                hi[e] = xh[i / 2][i % 2 * 4 + e];
+                lo[e] = xl[i / 2][i % 2 * 4 + e];
             }
             const int row = i * 16 + q * 4 + (r & 3);
             unsigned char *p = lds + row * XROW + (((wave * 2 + (r >> 3)) ^ (row & 15)) << 4) + ((r >> 2) & 1) * 8;
@@ -783,7 +812,6 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
             *(f16x4 *)(p + XLO) = or_transpose4(lo, lane);
         }
         __syncthreads();
-        f32x4 t[TILES];
 #pragma unroll
         for (int k = 0; k < TILES; k++) {
             t[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -797,30 +825,34 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
                                   *(const f16x8 *)(left + XLO + u));
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) t[k][e] = (t[k][e] + small[e]) * a.s[s].gram;
+            for (int e = 0; e < 4; e++) t[k][e] += small[e];
         }
-        __syncthreads();
+    };
+    // X = p(A) X, A from t; nothing else may be using the LDS
+    auto apply = [&](const auto &p) {
 #pragma unroll
-        for (int k = 0; k < TILES; k++)
+        for (int k = 0; k < TILES; k++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) t[k][e] *= p.gram;
             if (wave + k * NW < NT) or_small_store<MT>(lds, t[k], ti[k], tj[k], lane);
+        }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < TILES; k++) {
             if (wave + k * NW >= NT) continue;
-            f32x4 v, small = {0.f, 0.f, 0.f, 0.f};
+            f32x4 v = {0.f, 0.f, 0.f, 0.f}, small = v;
+            const unsigned char *left = lds + (ti[k] * 16 + r) * Rows::ROW, *right = lds + (tj[k] * 16 + r) * Rows::ROW;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = a.s[s].cb * t[k][e] + (ti[k] == tj[k] && q * 4 + e == r ? a.s[s].ca : 0.f);
-            if (a.s[s].square) {
-                const unsigned char *left = lds + (ti[k] * 16 + r) * Rows::ROW, *right = lds + (tj[k] * 16 + r) * Rows::ROW;
-#pragma unroll
-                for (int c = 0; c < MT / 2; c++) {
-                    const int u = ((c * 4 + q) ^ sw) << 4;
-                    or_small_multiply(v, small, *(const f16x8 *)(right + u), *(const f16x8 *)(right + Rows::LO + u), *(const f16x8 *)(left + u),
-                                      *(const f16x8 *)(left + Rows::LO + u));
-                }
+            for (int c = 0; c < MT / 2; c++) {
+                const int u = ((c * 4 + q) ^ sw) << 4;
+                or_small_multiply(v, small, *(const f16x8 *)(right + u), *(const f16x8 *)(right + Rows::LO + u), *(const f16x8 *)(left + u),
+                                  *(const f16x8 *)(left + Rows::LO + u));
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (v[e] + small[e]) * a.s[s].poly;
+            for (int e = 0; e < 4; e++) {
+                const float line = p.cb * t[k][e] + (ti[k] == tj[k] && q * 4 + e == r ? p.ca : 0.f);
+                v[e] = (p.square ? line + (v[e] + small[e]) : line) * p.poly;
+            }
             or_small_store<MT>(lds + Rows::REGION, v, ti[k], tj[k], lane);
         }
         __syncthreads();
@@ -834,17 +866,54 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
                 or_small_multiply(v, small, *(const f16x8 *)(left + u), *(const f16x8 *)(left + Rows::LO + u), xh[c], xl[c]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = (v[e] + small[e]) * a.s[s].apply;
+            for (int e = 0; e < 4; e++) x[i][e] = (v[e] + small[e]) * p.apply;
             if constexpr (MT * NW > 64) __builtin_amdgcn_sched_barrier(0);     // or too many fragments are read ahead for the registers
         }
-        __syncthreads();     // before the next step's X takes the place of M
+        __syncthreads();     // before the next X takes the place of M
+    };
+
+    if constexpr (!WIDE) {
+        load();
+        for (int s = 0; s < a.steps; s++) {
+            split();
+            gram();
+            __syncthreads();
+            apply(a.s[s]);
+        }
+    } else {
+        float *dump = a.x + ((long long)b * strips + strip) * (MT * NW * 256) + tid * 4;
+        if (a.launch == 0) load();
+        else {
+#pragma unroll
+            for (int i = 0; i < MT; i++) x[i] = *(const f32x4 *)(dump + i * (NW * 256));
+            const float *in = a.gram[a.launch & 1] + (long long)b * strips * (NT * 256) + lane * 4;
+#pragma unroll
+            for (int k = 0; k < TILES; k++) t[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < strips; s++)
+#pragma unroll
+                for (int k = 0; k < TILES; k++)
+                    if (wave + k * NW < NT) t[k] += *(const f32x4 *)(in + ((long long)s * NT + wave + k * NW) * 256);
+            split();
+            apply(a.s[a.launch - 1]);
+        }
+        if (a.launch < a.steps) {
+            split();
+            gram();
+            float *out = a.gram[(a.launch & 1) ^ 1] + ((long long)b * strips + strip) * (NT * 256) + lane * 4;
+#pragma unroll
+            for (int k = 0; k < TILES; k++)
+                if (wave + k * NW < NT) *(f32x4 *)(out + (wave + k * NW) * 256) = t[k];
+#pragma unroll
+            for (int i = 0; i < MT; i++) *(f32x4 *)(dump + i * (NW * 256)) = x[i];
+            return;
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         const int m = i * 16 + q * 4, count = n < a.n ? min(max(a.m - m, 0), 4) : 0;
         const long long at = a.flip ? n * a.ldo + m : m * a.ldo + n, step = a.flip ? 1 : a.ldo;
         if constexpr (STEP) {
-            float *o = (float *)a.out.p[blockIdx.x] + at;
+            float *o = (float *)a.out.p[b] + at;
             f32x4 p = or_small_load(o, step, count);
 #pragma unroll
             for (int e = 0; e < 4; e++) p[e] = p[e] * a.decay - a.rate * x[i][e];
@@ -853,7 +922,7 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
             bf16x4 v;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = (bf16_t)x[i][e];
-            or_small_write((bf16_t *)a.out.p[blockIdx.x] + at, step, count, v);
+            or_small_write((bf16_t *)a.out.p[b] + at, step, count, v);
         }
     }
 }
@@ -864,7 +933,10 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
 struct OrPlan {
     int m, n, flip;                          // short and long side; flip: the matrix has more rows than columns
     size_t x, xt, sq, total;                 // bytes per matrix: X, X^T, one m x m operand; all of it
+    int few, mt, strips;                     // few rows: or_small_kernel's, 16-row tiles and strips of OR_STRIP columns
 };
+
+constexpr int OR_STRIP = 256;
 
 static OrPlan or_plan(int rows, int cols) {
     OrPlan p;
@@ -875,6 +947,11 @@ static OrPlan or_plan(int rows, int cols) {
     p.xt = (size_t)p.n * or_split_ld(p.m);
     p.sq = (size_t)p.m * or_split_ld(p.m);
     p.total = p.x + 2 * p.xt + 5 * p.sq + (OR_PARTS + 1) * sizeof(double);     // with the norm's parts and rho
+    p.few = p.m <= 128 && p.n <= 16 * OR_STRIP;
+    p.mt = p.m <= 64 ? 4 : p.m <= 96 ? 6 : 8;
+    p.strips = (p.n + OR_STRIP - 1) / OR_STRIP;
+    const size_t wide = OR_PARTS * sizeof(double) + (size_t)p.strips * (p.mt * 16 * OR_STRIP + p.mt * (p.mt + 1) * 256) * sizeof(float);
+    if (p.few && p.strips > 1 && p.total < wide) p.total = wide;
     return p;
 }
 
@@ -987,25 +1064,28 @@ static OrPoly or_poly(const OrStep &s, int ea) {
     return p;
 }
 
-template <typename T, bool STEP, int MT, int NW>
+template <typename T, bool STEP, int MT, int NW, bool WIDE>
 static int or_launch_small(const OrSmall &a, int batch, hipStream_t stream) {
     constexpr int X = MT * 16 * NW * 64, AM = 2 * OrSmallRows<MT>::REGION, LDS = X > AM ? X : AM;
-    if (!lds_attr((const void *)or_small_kernel<T, STEP, MT, NW>, LDS)) return SGCLIP_ELAUNCH;
-    or_small_kernel<T, STEP, MT, NW><<<dim3(batch), 64 * NW, LDS, stream>>>(a);
+    static_assert(!WIDE || NW * 16 == OR_STRIP, "a strip per workgroup");
+    if (!lds_attr((const void *)or_small_kernel<T, STEP, MT, NW, WIDE>, LDS)) return SGCLIP_ELAUNCH;
+    const dim3 grid = WIDE ? dim3(ceil_div(a.n, OR_STRIP), batch) : dim3(batch);
+    or_small_kernel<T, STEP, MT, NW, WIDE><<<grid, 64 * NW, LDS, stream>>>(a);
     return launch_check("sgclip_orthogonalize");
 }
 
-// Up to 128 x 256, step by step.
+// Up to 128 x 4096, step by step.
 template <typename T, bool STEP>
-static int or_run_small(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
-                        hipStream_t stream) {
+static int or_run_few(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
+                      unsigned char *ws, hipStream_t stream) {
+    const OrPlan plan = or_plan(in.rows, in.cols);
     OrSmall a{};
     a.in = in;
     a.out = out;
     a.ldo = ldo;
-    a.flip = in.rows > in.cols;
-    a.m = a.flip ? in.cols : in.rows;
-    a.n = a.flip ? in.rows : in.cols;
+    a.flip = plan.flip;
+    a.m = plan.m;
+    a.n = plan.n;
     a.steps = sch.steps;
     a.scale = or_pow2(sch.ex[0]);
     a.eps = eps;
@@ -1021,9 +1101,23 @@ static int or_run_small(const OrInput &in, const OrPointers &out, long long ldo,
         a.s[k].square = p.square;
         a.s[k].apply = or_pow2((k + 1 < sch.steps ? sch.ex[k + 1] : 0) - s.em - sch.ex[k]);
     }
-    if (a.m <= 64) return a.n <= 128 ? or_launch_small<T, STEP, 4, 8>(a, batch, stream) : or_launch_small<T, STEP, 4, 16>(a, batch, stream);
-    if (a.m <= 96) return a.n <= 128 ? or_launch_small<T, STEP, 6, 8>(a, batch, stream) : or_launch_small<T, STEP, 6, 16>(a, batch, stream);
-    return a.n <= 128 ? or_launch_small<T, STEP, 8, 8>(a, batch, stream) : or_launch_small<T, STEP, 8, 16>(a, batch, stream);
+    if (plan.strips == 1) {
+        if (plan.mt == 4) return a.n <= 128 ? or_launch_small<T, STEP, 4, 8, false>(a, batch, stream) : or_launch_small<T, STEP, 4, 16, false>(a, batch, stream);
+        if (plan.mt == 6) return a.n <= 128 ? or_launch_small<T, STEP, 6, 8, false>(a, batch, stream) : or_launch_small<T, STEP, 6, 16, false>(a, batch, stream);
+        return a.n <= 128 ? or_launch_small<T, STEP, 8, 8, false>(a, batch, stream) : or_launch_small<T, STEP, 8, 16, false>(a, batch, stream);
+    }
+    double *parts = (double *)ws;
+    a.parts = parts;
+    a.x = (float *)(parts + (size_t)OR_PARTS * batch);
+    a.gram[0] = a.x + (size_t)batch * plan.strips * plan.mt * 16 * OR_STRIP;
+    a.gram[1] = a.gram[0] + (size_t)batch * plan.strips * plan.mt * (plan.mt + 1) / 2 * 256;
+    or_norm_kernel<T, STEP><<<dim3(OR_PARTS, batch), 256, 0, stream>>>(in, parts);
+    int rc = launch_check("sgclip_orthogonalize");
+    for (a.launch = 0; a.launch <= a.steps && rc == SGCLIP_OK; a.launch++)
+        rc = plan.mt == 4   ? or_launch_small<T, STEP, 4, 16, true>(a, batch, stream)
+             : plan.mt == 6 ? or_launch_small<T, STEP, 6, 16, true>(a, batch, stream)
+                            : or_launch_small<T, STEP, 8, 16, true>(a, batch, stream);
+    return rc;
 }
 
 // One launch group of up to OR_BATCH matrices.  in: gradients (and momentum buffers); out: bf16 results or parameters.
@@ -1031,8 +1125,10 @@ template <typename T, bool STEP>
 static int or_run(const OrInput &in, const OrPointers &out, long long ldo, int batch, const OrSchedule &sch, float eps, float decay, float rate,
                   unsigned char *ws, hipStream_t stream) {
     const OrPlan p = or_plan(in.rows, in.cols);
-    // as far as X and the squares fit a CU's LDS and registers; there it is faster at every size and number (above)
-    if (p.m <= 128 && p.n <= 256) return or_run_small<T, STEP>(in, out, ldo, batch, sch, eps, decay, rate, stream);
+    // One workgroup: at every size and number. Strips: while they fill the chip once (16 of 127 x 4000 225 us, by launches of
+    // or_gemm_kernel 320; 40 of them 578, 475), up to 64 rows always (40 of 64 x 4000 192, 360).
+    if (p.few && (p.strips == 1 || p.mt == 4 || batch * p.strips <= device_cus()))
+        return or_run_few<T, STEP>(in, out, ldo, batch, sch, eps, decay, rate, ws, stream);
     unsigned char *X = ws, *XT = X + p.x * batch, *XT2 = XT + p.xt * batch, *A = XT2 + p.xt * batch, *M = A + p.sq * batch, *Tm = M + p.sq * batch,
                   *Q = Tm + p.sq * batch, *Q2 = Q + p.sq * batch;
     double *parts = (double *)(Q2 + p.sq * batch);

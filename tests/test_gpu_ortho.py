@@ -168,7 +168,8 @@ def test_small_matrices(m, n):
         g = spectrum("gaussian", rows, cols, 3)
         want = iterate(g)
         tol = tolerance(rows, cols, want / math.sqrt(3))
-        assert rel(raw(g), want) <= tol
+        got = raw(g)
+        assert rel(got, want) <= tol and torch.equal(raw(g), got)
         for dtype in (F32, BF16):
             assert rel(G.orthogonalize(g.to(dtype)), iterate(g.to(dtype))) <= tol + UBF
         p, buf = torch.randn(3, rows, cols, device="cuda"), torch.randn(3, rows, cols, device="cuda")
@@ -181,6 +182,25 @@ def test_small_matrices(m, n):
         # momentum: three fp32 operations on each element; parameters: the direction's tolerance and three operations
         assert (buf.double() - mom).norm() <= 4 * U32 * (buf.double().norm() + g.double().norm())
         assert (p.double() - wantp).norm() <= 0.05 * 2 * tol * o.norm() + 4 * U32 * (before + o.norm())
+
+
+@pytest.mark.parametrize("m", [3, 40, 64, 70, 96, 100, 128])
+@pytest.mark.parametrize("n", [300, 512, 1030, 4096, 4097])
+def test_few_rows_in_strips(m, n):
+    """A workgroup per 256 columns, and what has too many of them: both orientations and types, the same bits at every call."""
+    for rows, cols in ((m, n), (n, m)):
+        for batch in (2, 20):
+            g = spectrum("gaussian", rows, cols, batch)
+            want = iterate(g)
+            tol = tolerance(rows, cols, want / math.sqrt(batch))
+            got = raw(g)
+            assert rel(got, want) <= tol and max(rel(a, b) for a, b in zip(got, want)) <= 3 * tol
+            assert torch.equal(raw(g), got)
+        x = g[:2].to(BF16)
+        y = G.orthogonalize(x)
+        assert rounded(y, iterate(x), tol)
+        for _ in range(3):
+            assert torch.equal(G.orthogonalize(x), y)
 
 
 @pytest.mark.parametrize("rows,cols", [(150, 200), (700, 300)])
