@@ -21,15 +21,16 @@ def _stream(t: Optional[torch.Tensor] = None) -> int:
     kernel will touch: its device must be the current one (HIP launches on the current device; a pointer of
     another GPU would fault there), so callers with tensors elsewhere run under `torch.cuda.device(...)`,
     as PredicateModel does for its own device."""
-    device = torch.cuda.current_device()
+    # the runtime's own answers where torch hands them out: a Stream object costs 2 us, as much as a launch
+    device = _CURRENT_DEVICE() if t is not None and _CURRENT_DEVICE is not None else torch.cuda.current_device()
     if t is not None and t.device.index != device:
         raise RuntimeError(f"tensor on {t.device} but the current HIP device is cuda:{device}: "
                            f"run this call under torch.cuda.device({t.device.index})")
-    # the handle itself where torch hands it out: a Stream object costs 2 us, as much as a launch
     return _RAW_STREAM(device) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None)     # without torch.cuda's check that the runtime is up: a tensor on it is proof
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -352,9 +353,10 @@ def _rows2d(name: str, t: torch.Tensor, dtypes) -> int:
 
 
 def _same_device(a: torch.Tensor, *others: Optional[torch.Tensor]):
+    device = a.device
     for t in others:
-        if t is not None and t.device != a.device:
-            raise ValueError(f"tensors on different devices: {a.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
 
 
 def _byte_range(t: torch.Tensor):
