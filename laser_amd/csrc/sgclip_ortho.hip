@@ -616,8 +616,8 @@ __global__ __launch_bounds__(256) void or_split_kernel(OrInput a, const double *
 // result and, with the columns of M in the same order (32 of them: four of the first 16, then four of the second), takes its
 // second operand, so that M X needs nothing of X but registers.  For A = X X^T the waves lay out X's rows in LDS, then A, then M; the
 // lower 16 x 16 tiles of A and M are computed and written to both sides.
-// Bound by one CU: 128 x 256 take 3.5 us a step on its matrix pipe and as long to read their fragments from LDS, between five
-// barriers.  Against the launches of or_gemm_kernel, us: 4 of 33 x 64 18 (67), of 64 x 64 19 (68), of 65 x 255 39 (85), of 128 x 128 45
+// Bound by one CU: of the 12 us of a step of 127 x 255, 5.4 are its matrix pipe's and 7.7 the LDS's (fragments, mostly of A and M),
+// between five barriers.  Against the launches of or_gemm_kernel, us: 4 of 33 x 64 18 (67), of 64 x 64 19 (68), of 65 x 255 39 (85), of 128 x 128 45
 // (79), of 127 x 255 66 (86); 200 of them 284 (442).  In strips: 4 of 64 x 513 46 (89), of 64 x 2000 55 (136), of 96 x 1023 72 (116), of
 // 127 x 513 96 (97), of 127 x 2000 128 (163).
 // A product's results are used in its own block of instructions, never behind a branch beside it: the compiler leaves the wait for the

@@ -13,7 +13,7 @@ import pytest
 import torch
 from torch import nn
 
-from laser_amd import _lib, grad_ops as G, ops, training
+from laser_amd import grad_ops as G, ops, training
 
 pytestmark = pytest.mark.gpu
 
