@@ -5,9 +5,12 @@
 //   * every m x m product is computed on the tiles of one triangle and written to both;
 //   * several steps need X only once: M_i = p(A_i), Q <- M_i Q, A_{i+1} = M_i A_i M_i, then X <- Q X.  A block of k steps costs
 //     3 m^2 n + (4 k - 3) m^3 multiplications and additions instead of k (3 m^2 n + m^3).
-// The price of a block is precision, since A holds the squares of the singular values: against 64 bits the result of five
-// steps is off by 1e-6 (relative, before its rounding) step by step and by 2e-6 (gaussian matrices) to 3e-4 as one block (power-law,
-// exponential and low-rank spectra).  Blocks are at most five steps long, and only used where they save time.
+// The price of a block is precision: a rounding of A grows by a^2 with every A_{i+1} = M_i A_i M_i, where a step from X makes a new A.
+// Two steps on one A cost nothing that shows: emulated over 25 spectra of 256 x 512 and 512 x 1024, |X| = 1 at the start, the result of
+// five steps is off by at most 1.0e-4 (Frobenius norm, before its rounding) step by step, 8.3e-5 in blocks of two, 9.7e-5 in plain fp32;
+// with a block of three first 2.3e-4, all five on one A 6.1e-3, and with coefficients as steep as 4.08, -6.89, 2.93 1.3e-3 and 7.1e-2.
+// So blocks are two steps long, and only used where they save time.  On the GPU, against plain fp32 over seven spectra of seven sizes
+// from 128 x 256 to 1024 x 4096: 0.4 to 1.5 times its error, at most 1.2e-4 (1.9e-4).
 //
 // Precision.  The first steps multiply small singular values by a each, 485 times over five steps with the usual coefficients,
 // and rounding errors with them: with bf16 products the result is off by 2 to 20 %, with fp16 by 0.2 to 3 %.  Operands are
@@ -144,7 +147,7 @@ __device__ __forceinline__ void or_store_cols(const f32x4 (&v)[SM], unsigned cha
 }
 
 // A 16 x 16 block on the diagonal of a symmetric result, made exactly symmetric from its lower triangle.  What is left of
-// asymmetry grows from step to step (the error of five steps on one Gram matrix: 1e-5 with it, 1e-3 to 2e-2 without).
+// asymmetry grows from step to step of a block (five on one Gram matrix were off by 1e-5 with it, by 1e-3 to 2e-2 without).
 __device__ __forceinline__ void or_symmetrize(f32x4 &v, unsigned char *region, int lane) {
     const int r = lane & 15, q = lane >> 4;
     float *buf = (float *)region;
@@ -977,8 +980,10 @@ struct OrSchedule {
 
 static bool or_schedule(const float *coefficients, int steps, int m, int n, OrSchedule &o) {
     o.steps = steps;
-    // blocks save nothing for square matrices, and next to nothing where the launches' latency counts; single steps lose least
-    const int most = n * 4LL < m * 5LL || m < 256 ? 1 : 5;
+    // Two steps at most (the head of this file says why), where they save time: updates in us, two steps on one Gram matrix against single
+    // ones, 24 of 256 x 512 166 and 171, of 512 x 1024 589 and 596, of 1024 x 2048 2511 and 2829, of 1024 x 4096 4015 and 5179; but 24 of
+    // 512 x 640 480 and 427, one of 768 x 1152 207 and 190, 24 of 200 x 400 149 and 151, one of them 112 and 105 (more launches)
+    const int most = n < 2LL * m || m < 256 ? 1 : 2;
     o.blocks = (steps + most - 1) / most;
     for (int i = 0; i < o.blocks; i++) o.len[i] = steps / o.blocks + (i < steps % o.blocks);
     double top = 1.0, qb = 1.0;     // bounds of the singular values (1 after the normalisation) and of Q
