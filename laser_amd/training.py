@@ -17,11 +17,13 @@ parameter gradients.
 """
 from __future__ import annotations
 
+import weakref
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 import torch
 from torch import nn
+from torch.utils.weak import WeakTensorKeyDictionary
 
 from . import _lib, grad_ops as G, ops
 from .config import ClipConfig
@@ -256,6 +258,8 @@ class GradSink:
     def __init__(self, tower: TrainTower):
         self.tower = tower
         self.flat = tower.flat
+        if self.flat is not None:
+            self.flat.attach_gradients()     # or what was dropped, not zeroed, would go on summing where no `.grad` shows it
         self.loose: Dict[str, torch.Tensor] = {}
 
     def get(self, name: str) -> torch.Tensor:
@@ -290,6 +294,10 @@ class GradSink:
         return out
 
 
+# parameter -> (weak reference to its FlatParameters, its name there)
+_flat_place = WeakTensorKeyDictionary()
+
+
 class FlatParameters:
     """All parameters of a module in ONE fp32 buffer and their gradients in a second one.
 
@@ -311,12 +319,14 @@ class FlatParameters:
         self.data = torch.zeros(off, dtype=F32, device=dev)
         self.grad = torch.zeros(off, dtype=F32, device=dev)
         self.params = [p for _, p in named_params]
+        here = weakref.ref(self)
         with torch.no_grad():
             for n, p in named_params:
                 o, cnt, shape = self.index[n]
                 self.data[o:o + cnt].copy_(p.detach().reshape(-1))
                 p.data = self.data[o:o + cnt].view(shape)
                 p.grad = self.grad[o:o + cnt].view(shape)
+                _flat_place[p] = (here, n)
 
     def grad_view(self, name: str) -> torch.Tensor:
         o, cnt, shape = self.index[name]
@@ -336,6 +346,15 @@ class FlatParameters:
         for n, p in zip(self.index, self.params):    # re-attach views a foreign zero_grad(set_to_none=True) dropped
             if p.grad is None:
                 p.grad = self.grad_view(n)
+
+    def attach_gradients(self):
+        """Where a foreign zero_grad(set_to_none=True) dropped a view: its place in the buffer becomes zeros, and `.grad` again."""
+        dropped = [(n, p) for n, p in zip(self.index, self.params) if p.grad is None]
+        if dropped:
+            views = [self.grad_view(n) for n, _ in dropped]
+            torch._foreach_zero_(views)
+            for (_, p), v in zip(dropped, views):
+                p.grad = v
 
     def mark_updated(self):
         for p in self.params:
@@ -545,6 +564,24 @@ def linear_mxfp4(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 # ---------------------------------------------------------------------------------------------
 # optimizer and gradient exchange
 # ---------------------------------------------------------------------------------------------
+def _zero_gradients(params, set_to_none: bool):
+    """zero_grad of an optimiser of single parameters.  One that lies in a `FlatParameters` keeps its view of the gradient buffer, which
+    the towers' backward adds to and the all-reduce sends, and has it zeroed; set_to_none holds for the others."""
+    zero = []
+    for p in params:
+        at = _flat_place.get(p) if len(_flat_place) else None
+        flat = at[0]() if at is not None else None
+        if flat is not None:
+            p.grad = flat.grad_view(at[1])
+        elif set_to_none:
+            p.grad = None
+        if p.grad is not None:
+            zero.append(p.grad)
+    if zero:
+        with torch.no_grad():
+            torch._foreach_zero_(zero)
+
+
 class Adam:
     """torch.optim.Adam's update (scripts/train_sgclip.py:232-241 uses its defaults: betas (0.9, 0.999),
     eps 1e-8, no weight decay) as HIP kernel launches: one per parameter, or ONE over the whole buffer when
@@ -566,11 +603,7 @@ class Adam:
         if self.flat is not None:
             self.flat.zero_grad()
             return
-        for p in self.params:
-            if set_to_none:
-                p.grad = None
-            elif p.grad is not None:
-                p.grad.zero_()
+        _zero_gradients(self.params, set_to_none)
 
     @torch.no_grad()
     def step(self):
@@ -606,7 +639,7 @@ class Muon:
 
     Matrices of one shape take their launches together; their momenta lie in one buffer per shape (`momentum`, in the order
     `groups` lists).  Parameters without a gradient are left as they are.  With `FlatParameters` the matrices are the
-    parameters themselves (their `.grad` are views of the flat buffer):
+    parameters themselves; their `.grad` are views of the flat buffer, and `zero_grad` fills them with zeros whatever it is told:
 
         matrices, rest = split_for_muon(model.named_parameters())
         opts = Muon(matrices, lr=2e-4), Adam(rest, lr=1e-5)
@@ -631,11 +664,7 @@ class Muon:
         self.momentum = [torch.zeros((len(g),) + tuple(g[0].shape), dtype=F32, device=g[0].device) for g in self.groups]
 
     def zero_grad(self, set_to_none: bool = True):
-        for p in self.params:
-            if set_to_none:
-                p.grad = None
-            elif p.grad is not None:
-                p.grad.zero_()
+        _zero_gradients(self.params, set_to_none)
 
     @torch.no_grad()
     def step(self):
@@ -754,6 +783,7 @@ class GradientReducer:
 
     def begin(self):
         """Start of a step (before forward)."""
+        self.flat.attach_gradients()
         self._ready, self._launched, self._pending = set(), 0, []
         for t in self.towers:
             t.backward_pending = 0     # forward passes without a backward (scoring under no_grad) count for nothing
