@@ -348,13 +348,20 @@ class FlatParameters:
                 p.grad = self.grad_view(n)
 
     def attach_gradients(self):
-        """Where a foreign zero_grad(set_to_none=True) dropped a view: its place in the buffer becomes zeros, and `.grad` again."""
-        dropped = [(n, p) for n, p in zip(self.index, self.params) if p.grad is None]
+        """Makes every `.grad` its view again.  Where a foreign zero_grad(set_to_none=True) dropped it, the place in the buffer becomes
+        zeros; what has been put there since (by autograd, for a parameter outside the towers) moves into the buffer."""
+        dropped, base = [], self.grad.data_ptr()
+        for (n, (o, _, _)), p in zip(self.index.items(), self.params):
+            g = p.grad
+            if g is None:
+                p.grad = self.grad_view(n)
+                dropped.append(p.grad)
+            elif g.data_ptr() != base + 4 * o:
+                p.grad = self.grad_view(n)
+                with torch.no_grad():
+                    p.grad.copy_(g)
         if dropped:
-            views = [self.grad_view(n) for n, _ in dropped]
-            torch._foreach_zero_(views)
-            for (_, p), v in zip(dropped, views):
-                p.grad = v
+            torch._foreach_zero_(dropped)
 
     def mark_updated(self):
         for p in self.params:
@@ -610,6 +617,7 @@ class Adam:
         self.step_count += 1
         b1, b2 = self.betas
         if self.flat is not None:
+            self.flat.attach_gradients()
             G.adamw(self.flat.data, self.flat.grad, self.m, self.v, self.step_count, self.lr, b1, b2, self.eps,
                     self.weight_decay)
             self.flat.mark_updated()

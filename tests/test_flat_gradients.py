@@ -81,3 +81,31 @@ def test_a_reduced_step_starts_with_every_view_in_place():
     assert all(is_place(flat, n, p) and not p.grad.any() for n, p in named)
     (named[3][1] * 5).backward()                     # a parameter whose gradient autograd adds
     assert flat.grad_view("m.logit_scale").item() == 5.0
+
+
+def test_a_gradient_beside_the_buffer_moves_into_it():
+    """torch's zero_grad, then a backward pass: autograd gives a parameter outside the towers a tensor of its own."""
+    named, flat = flattened()
+    scale = named[3][1]
+    for _, p in named:
+        p.grad = None
+    (scale * 5).backward()
+    assert not is_place(flat, "m.logit_scale", scale)
+    training.GradSink(types.SimpleNamespace(flat=flat, flat_prefix="m."))
+    assert all(is_place(flat, n, p) for n, p in named)
+    assert scale.grad.item() == 5.0 and not named[0][1].grad.any()
+    (scale * 2).backward()
+    assert flat.grad_view("m.logit_scale").item() == 7.0
+
+
+def test_flat_adam_reads_every_gradient(monkeypatch):
+    named, flat = flattened()
+    opt = training.Adam(flat)
+    seen = []
+    monkeypatch.setattr(training.G, "adamw", lambda p, g, *a: seen.append(g.clone()))
+    for _, p in named:
+        p.grad = None
+    (named[3][1] * 5).backward()
+    opt.step()
+    for n, (at, count, _) in flat.index.items():       # what lies between them, for alignment, is no parameter's
+        assert seen[0][at:at + count].sum().item() == (5.0 if n == "m.logit_scale" else 0.0)
