@@ -73,7 +73,7 @@ struct OrGemm {
     long long sL, sR, sO, sOT, sA;     // bytes from one matrix of the batch to the next
     float alpha[2];                    // from the accumulator's scale to the output's
     float ca, cb;                      // OR_POLY: out = alpha (ca I + cb A + A A), the first two in the accumulators from the start
-    float decay, rate;                 // OR_UPDATE: p = decay p - rate out
+    float decay, rate;                 // OR_UPDATE: p = decay p - rate out, rounded twice: decay p, and the whole (alpha is a power of two)
     long long ldo;                     // OR_OUT / OR_UPDATE: row stride in elements
     int M, N, kc, ldl, ldr;            // rows of L, rows of R, stages (0: none), bytes of their rows
     int tiles_m, tiles_n, wide;
@@ -393,15 +393,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void or_gemm_kernel(OrGemm g) {
                     float *o = (float *)g.out.p[b] + at;
                     if (g.wide) {
                         float4 w = *(const float4 *)o;
-                        w.x = w.x * g.decay - g.rate * (v[0] * alpha);
-                        w.y = w.y * g.decay - g.rate * (v[1] * alpha);
-                        w.z = w.z * g.decay - g.rate * (v[2] * alpha);
-                        w.w = w.w * g.decay - g.rate * (v[3] * alpha);
+                        w.x = fmaf(-g.rate, v[0] * alpha, w.x * g.decay);
+                        w.y = fmaf(-g.rate, v[1] * alpha, w.y * g.decay);
+                        w.z = fmaf(-g.rate, v[2] * alpha, w.z * g.decay);
+                        w.w = fmaf(-g.rate, v[3] * alpha, w.w * g.decay);
                         *(float4 *)o = w;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (n + e < g.N) o[e] = o[e] * g.decay - g.rate * (v[e] * alpha);
+                            if (n + e < g.N) o[e] = fmaf(-g.rate, v[e] * alpha, o[e] * g.decay);
                     }
                 }
             }
@@ -455,7 +455,7 @@ struct OrInput {
 template <typename T, bool STEP>
 __device__ __forceinline__ float or_direction(const OrInput &a, float g, float buf) {
     if constexpr (!STEP) return g;
-    return a.nesterov ? (1.0f - a.mu) * g + a.mu * buf : buf;
+    return a.nesterov ? fmaf(a.mu, buf, (1.0f - a.mu) * g) : buf;
 }
 
 template <typename T>
@@ -486,10 +486,10 @@ __global__ __launch_bounds__(256) void or_norm_kernel(OrInput a, double *__restr
             float *bp = buf + i * step;
             if (a.vec) m = *(const float4 *)bp;
             else m.x = *bp;
-            m.x = a.mu * m.x + (1.0f - a.mu) * v.x;
-            m.y = a.mu * m.y + (1.0f - a.mu) * v.y;
-            m.z = a.mu * m.z + (1.0f - a.mu) * v.z;
-            m.w = a.mu * m.w + (1.0f - a.mu) * v.w;
+            m.x = fmaf(a.mu, m.x, (1.0f - a.mu) * v.x);
+            m.y = fmaf(a.mu, m.y, (1.0f - a.mu) * v.y);
+            m.z = fmaf(a.mu, m.z, (1.0f - a.mu) * v.z);
+            m.w = fmaf(a.mu, m.w, (1.0f - a.mu) * v.w);
             if (a.vec) *(float4 *)bp = m;
             else *bp = m.x;
         }
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
                 f32x4 v = or_small_load(bp, step, count);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    if constexpr (!WIDE) v[e] = a.in.mu * v[e] + (1.0f - a.in.mu) * x[i][e];      // (WIDE: done with the norm)
+                    if constexpr (!WIDE) v[e] = fmaf(a.in.mu, v[e], (1.0f - a.in.mu) * x[i][e]);      // (WIDE: done with the norm)
                     x[i][e] = or_direction<T, STEP>(a.in, x[i][e], v[e]);
                 }
                 if constexpr (!WIDE) or_small_write(bp, step, count, v);
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(64 * NW) void or_small_kernel(OrSmall a) {
             float *o = (float *)a.out.p[b] + at;
             f32x4 p = or_small_load(o, step, count);
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = p[e] * a.decay - a.rate * x[i][e];
+            for (int e = 0; e < 4; e++) p[e] = fmaf(-a.rate, x[i][e], p[e] * a.decay);
             or_small_write(o, step, count, p);
         } else {
             bf16x4 v;
@@ -1356,8 +1356,8 @@ int sgclip_muon_step(float *const *params, const float *const *grads, float *con
             out.p[i] = params[b0 + i];
             in.vec = in.vec && (((uintptr_t)in.g.p[i] | (uintptr_t)in.buf.p[i]) & 15) == 0;
         }
-        rc = or_run<float, true>(in, out, cols, n, sch, eps, 1.0f - lr * weight_decay, lr * scale, (unsigned char *)workspace_dev,
-                                 (hipStream_t)stream);
+        rc = or_run<float, true>(in, out, cols, n, sch, eps, (float)(1.0 - (double)lr * weight_decay), (float)((double)lr * scale),
+                                 (unsigned char *)workspace_dev, (hipStream_t)stream);
     }
     return rc;
 }
