@@ -401,9 +401,9 @@ int sgclip_mxfp4_linear(const void *x_dev, int x_dtype, int64_t ldx, const void 
                         int K, int epilogue, const float *bias_dev, const float *aux_dev, int64_t ldaux, void *out_dev, int64_t ldo,
                         void *workspace_dev, size_t workspace_bytes, void *stream);
 
-/* The layer's gradients for dy bf16 or f32 [M, N] (row stride lddy), in the quantised operands: dx = dy w [M, K] (bf16 or f32), dw =
- * dy^T x f32 [N, K], db = the column sums of dy f32 [N]; contiguous, overwritten, NULL where not needed.  bf16 products of dy (rounded
- * if it is f32) with the operands, which bf16 holds exactly; dw is summed with atomics. */
+/* The layer's gradients for dy bf16 or f32 [M, N] (row stride lddy; N up to 2^22), in the quantised operands: dx = dy w [M, K] (bf16
+ * or f32), dw = dy^T x f32 [N, K], db = the column sums of dy f32 [N]; contiguous, overwritten, NULL where not needed.  bf16 products
+ * of dy (rounded if it is f32) with the operands, which bf16 holds exactly; dw is summed with atomics. */
 size_t sgclip_mxfp4_linear_bwd_workspace_bytes(const void *dy_dev, int dy_dtype, int64_t lddy, int M, int N, int K);
 int sgclip_mxfp4_linear_bwd(const void *dy_dev, int dy_dtype, int64_t lddy, const void *x_codes_dev, const void *x_scales_dev,
                             const void *w_codes_dev, const void *w_scales_dev, int M, int N, int K, void *dx_dev, int dx_dtype, float *dw_dev,

@@ -853,6 +853,8 @@ static void mx_zero(T *a, long long na, T *b, long long nb, hipStream_t st) {
 
 // workspace of the layer's gradients: zeros f32 [K]; dy bf16 [M][n64], if it has to be laid out; w^T bf16 [K][n64]; x bf16 [M][k8];
 // dw f32 [n8][k8], if it has to be cropped; column sums
+constexpr int MX_BWD_LD = 1 << 22;     // the products count 256 rows' bytes in 32 bits
+
 struct MxBwdPlan {
     int n8, n64, k8;
     bool pad, crop;
@@ -864,7 +866,7 @@ static MxBwdPlan mx_bwd_plan(const void *dy, int dtype, long long lddy, int M, i
     p.n8 = (N + 7) / 8 * 8;
     p.n64 = (N + 63) / 64 * 64;
     p.k8 = (K + 7) / 8 * 8;
-    p.pad = dtype == SGCLIP_DTYPE_F32 || N % 64 != 0 || lddy % 8 != 0 || lddy > 0x7fffffff || ((uintptr_t)dy & 15);
+    p.pad = dtype == SGCLIP_DTYPE_F32 || N % 64 != 0 || lddy % 8 != 0 || lddy > MX_BWD_LD || ((uintptr_t)dy & 15);
     p.crop = p.n8 != N || p.k8 != K;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1051,6 +1053,10 @@ int sgclip_mxfp4_linear_bwd(const void *dy_dev, int dy_dtype, int64_t lddy, cons
                             float *db_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
     const char *who = "sgclip_mxfp4_linear_bwd";
     if (!mx_shape_ok(who, M, K) || !mx_shape_ok(who, N, K)) return SGCLIP_EINVAL;
+    if (N > MX_BWD_LD) {
+        set_error("%s: N=%d is more than %d", who, N, MX_BWD_LD);
+        return SGCLIP_EINVAL;
+    }
     const hipStream_t st = (hipStream_t)stream;
     if (M == 0 || N == 0) {
         if (dx_dev && dx_dtype == SGCLIP_DTYPE_F32) mx_zero((float *)dx_dev, (long long)M * K, (float *)nullptr, 0, st);
