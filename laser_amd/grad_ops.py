@@ -282,11 +282,12 @@ def linear_mxfp4_bwd(dy: torch.Tensor, xq: Mxfp4, wq: Mxfp4, dx_dtype: torch.dty
 def linear_mxfp4_bwd_at(dy: torch.Tensor, operands, M: int, N: int, K: int, dx_dtype: torch.dtype, need_dx: bool, need_dw: bool, need_db: bool):
     """`linear_mxfp4_bwd`, unchecked, by the addresses of x's codes and scales and of the weight's (on dy's device)."""
     lib, dev = _lib.load(), dy.device
-    dy = dy.contiguous()
+    if (N > 1 and dy.stride(1) != 1) or (M > 1 and dy.stride(0) < N):      # rows that are strided themselves, or overlap
+        dy = dy.contiguous()
     dx = torch.empty((M, K), dtype=dx_dtype, device=dev) if need_dx else None
     dw = torch.empty((N, K), dtype=F32, device=dev) if need_dw else None
     db = torch.empty(N, dtype=F32, device=dev) if need_db else None
-    head = (dy.data_ptr(), _dtype_code(dy), N)
+    head = (dy.data_ptr(), _dtype_code(dy), dy.stride(0) if M > 1 else N)
     need = lib.sgclip_mxfp4_linear_bwd_workspace_bytes(*head, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.check(lib.sgclip_mxfp4_linear_bwd(*head, *operands, M, N, K, _ptr(dx), _lib.DTYPE_F32 if dx_dtype == F32 else _lib.DTYPE_BF16,
