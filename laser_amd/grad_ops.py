@@ -327,14 +327,14 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, e
     table = _coefficients(coefficients, steps)
     if out is None:
         out = torch.empty(g.shape, dtype=BF16, device=g.device)
-    if g.numel() == 0:
-        return out
     if out.shape != g.shape or out.dtype != BF16:
         raise ValueError(f"orthogonalize: out must be bf16 {tuple(g.shape)}, got {out.dtype} {tuple(out.shape)}")
+    _same_device(g, out)
+    if g.numel() == 0:
+        return out
     for name, t in (("g", g), ("out", out)):
         if (cols > 1 and t.stride(-1) != 1) or (rows > 1 and t.stride(-2) < cols):
             raise ValueError(f"orthogonalize: rows of {name} must be contiguous and apart, got strides {t.stride()}")
-    _same_device(g, out)
     _apart("orthogonalize", out, g)
     ld = [t.stride(-2) if rows > 1 else cols for t in (g, out)]
     bs = [t.stride(0) if batch > 1 else rows * cols for t in (g, out)]
