@@ -422,7 +422,8 @@ int sgclip_column_sums(const void *in_dev, int in_dtype, int64_t ld, int M, int 
  * X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T on the shorter side: singular values
  * go towards 1, singular vectors stay.  coefficients: host f32 [steps][3] = a, b, c of every step.  Products of
  * operands in 22 bits (two fp16 halves) with fp32 sums: the result, before its rounding, is off by 0.4 to 1.5 times what it is
- * with fp32 products (49 pairs of size and spectrum).  coefficients under which values would leave fp16's range are refused.
+ * with fp32 products (49 pairs of size and spectrum).  Elements below 2^-39 of |G|_F +
+ * eps count as zero.  coefficients under which values would leave fp16's range are refused.
  * ---------------------------------------------------------------------- */
 size_t sgclip_orthogonalize_workspace_bytes(int batch, int rows, int cols);
 /* g bf16 or f32 [batch][rows][cols] (row stride ldg, batch stride batch_stride, elements; 1 <= rows, cols <= 65536) -> out bf16

@@ -383,8 +383,8 @@ __device__ __forceinline__ void mx_epilogue(const MxGemm &g, const f32x4 (&acc)[
 }
 
 // Tile of 2 WT x 2 WT, four waves of WT x WT (32 or 64) each; one 256-deep stage in flight behind the one computed, its scales
-// with it in registers, one barrier per stage.  Bound by the latency of a stage's fetch: 9232 x 768 x 768 9.2 us (scales loaded
-// where they are used, results four columns at a time: 12.6), 1540 x 768 x 768 3.9 us.
+// with it in registers, one barrier per stage.  Bound by the latency of a stage's fetch: 9232 x 768 x 768 9.6 us (scales loaded
+// where they are used, results four columns at a time: 12.6), 1540 x 768 x 768 4.8 us, added to a residual 6.0.
 template <int EPI, int WT>
 __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
     constexpr int T = 2 * WT, NT = WT / 16, OP = T * 128;
@@ -471,8 +471,9 @@ __global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemm g) {
 // and the DMA of stage g + 2 (of the next tile, if need be) starts into the slot just freed.  A tile's results leave from the registers
 // while the next tile's operands arrive; the barrier after them waits for the fetches only (they are older than the stores, and the
 // counter retires in order).
-// 73856 x 1024 x 4096 in 213 us (with GELU 244): 117 are the main loop alone (1.40 a stage, 1.08 at the matrix rate), 25 its fetches, the
-// rest the results, 3.7 a tile (GELU 5.4), behind which the next tile's fetches wait.  K = 4096: 612 us, 4.0 PFLOP/s.
+// 73856 x 1024 x 4096 in 209 us at the least, 226 on average of ten (with GELU 241 and 250).  Of 213 us 117 are the main loop alone (1.40 a
+// stage, 1.08 at the matrix rate), 25 its fetches, the rest the results, 3.7 a tile (GELU 5.4), behind which the next tile's fetches
+// wait.  K = 4096: 606 us at the least, 4.1 PFLOP/s, 646 on average.
 // ---------------------------------------------------------------------------
 constexpr int MXP_OP = 256 * 128, MXP_SLOT = 2 * MXP_OP + 4096, MXP_BIAS = 2 * MXP_SLOT, MXP_LDS = MXP_BIAS + 4096;
 static_assert(MXP_LDS <= 160 * 1024, "LDS of a CU");
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(1024) void mx_few_rows_kernel(const T *__restrict__
 // ---------------------------------------------------------------------------
 // Column sums without atomics (bias gradients): every workgroup sums a strip of rows of 512 columns (a lane eight of them, its
 // waves every WAVES-th row), a second launch adds the strips in a fixed order; few rows are one strip of 16 waves, and no second
-// launch.  Bound by HBM: 36928 x 4096 bf16 in 51 us (5.9 TB/s), the second launch 4 us.
+// launch.  Bound by HBM: 36928 x 4096 bf16 in 52 us (5.8 TB/s), the second launch 5 us.
 // ---------------------------------------------------------------------------
 constexpr int CS_COLS = 512, CS_STRIPS = 256, CS_ROWS = 32, CS_FEW = 512;
 

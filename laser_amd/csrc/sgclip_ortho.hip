@@ -19,9 +19,9 @@
 // bounds of the polynomial over the range of singular values.
 //
 // A bf16 matrix scaled by a power of two fits one fp16 half, and stays so ("plain") until the first block has been applied to it:
-// its Gram matrix is one product and Q X two (24 of 1024 x 4096: 157 us instead of 360 and 403 instead of 529, and 113 instead of
-// 195 to lay them out; 2.12 ms instead of 2.47 in all).  What the power leaves of 2^e / (|U| + eps), a factor rho in [1, 2) of
-// each matrix, multiplies the products' results.
+// its Gram matrix is one product and Q X two (24 of 1024 x 4096: 150 us instead of 289 and 420 instead of 554, and 110 instead of
+// 216 to lay them out; 3.45 ms instead of 3.72 in all, under a profiler).  What the power leaves of 2^e / (|U| + eps), a factor rho
+// in [1, 2) of each matrix, multiplies the products' results.
 //
 // Storage of an operand with K columns: "split rows" with row stride ceil(K / 32) * 128 bytes, per 32 columns 64 bytes of hi and
 // 64 of lo; "plain rows" of fp16 with row stride ceil(K / 64) * 128 bytes; zeros behind K.  A stage of the product's loop is one
