@@ -341,25 +341,30 @@ class FlatParameters:
             o += self.index[n][1]
         return self.grad[o0:o]
 
+    def _displaced(self):
+        """(parameter, its view, its present `.grad`) where that is not the view."""
+        base = self.grad.data_ptr()
+        for (n, (o, _, _)), p in zip(self.index.items(), self.params):
+            g = p.grad
+            if g is None or g.data_ptr() != base + 4 * o:
+                yield p, self.grad_view(n), g
+
     def zero_grad(self):
         self.grad.zero_()
-        for n, p in zip(self.index, self.params):    # re-attach views a foreign zero_grad(set_to_none=True) dropped
-            if p.grad is None:
-                p.grad = self.grad_view(n)
+        for p, view, _ in self._displaced():
+            p.grad = view
 
     def attach_gradients(self):
         """Makes every `.grad` its view again.  Where a foreign zero_grad(set_to_none=True) dropped it, the place in the buffer becomes
         zeros; what has been put there since (by autograd, for a parameter outside the towers) moves into the buffer."""
-        dropped, base = [], self.grad.data_ptr()
-        for (n, (o, _, _)), p in zip(self.index.items(), self.params):
-            g = p.grad
+        dropped = []
+        for p, view, g in self._displaced():
+            p.grad = view
             if g is None:
-                p.grad = self.grad_view(n)
-                dropped.append(p.grad)
-            elif g.data_ptr() != base + 4 * o:
-                p.grad = self.grad_view(n)
+                dropped.append(view)
+            else:
                 with torch.no_grad():
-                    p.grad.copy_(g)
+                    view.copy_(g)
         if dropped:
             torch._foreach_zero_(dropped)
 

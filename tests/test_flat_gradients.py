@@ -109,3 +109,15 @@ def test_flat_adam_reads_every_gradient(monkeypatch):
     opt.step()
     for n, (at, count, _) in flat.index.items():       # what lies between them, for alignment, is no parameter's
         assert seen[0][at:at + count].sum().item() == (5.0 if n == "m.logit_scale" else 0.0)
+
+
+def test_flat_zero_grad_clears_what_lies_beside_the_buffer():
+    named, flat = flattened()
+    for _, p in named:
+        p.grad = None
+    (named[3][1] * 5).backward()
+    flat.zero_grad()
+    assert all(is_place(flat, n, p) and not p.grad.any() for n, p in named)
+    (named[3][1] * 2).backward()
+    flat.attach_gradients()
+    assert named[3][1].grad.item() == 2.0
